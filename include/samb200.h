@@ -335,6 +335,83 @@ int samb_mask_stats(const void* logits, int is_bf16, int64_t N, int H, int W, fl
 int samb_mask_rle(const uint8_t* masks, int64_t N, int H, int W, int32_t* counts, int32_t* n_counts, int cap,
                   void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Operators of transformer blocks beside the reference's own kind (no counterpart in the reference): norms around a
+ * block, rotary positions, a mixture of experts.  16-bit tensors are bf16, or float16 when is_f16 != 0.
+ * ------------------------------------------------------------------------------------------- */
+
+/* The norms before and after a residual addition, with the block's gate and the residual's scale:
+ *   x_new = res_scale * residual + gate * post(h),   y = pre(x_new)
+ * over rows of C elements (C % 8 == 0, C <= 8192).  post / pre: LayerNorm, or x / sqrt(mean(x^2) + eps) when rms != 0,
+ * with fp32 gain and optional offset; a null post_gamma leaves h as it is, a null pre_gamma (with a null y) leaves y
+ * out.  gate: null, or gate_rows vectors of C fp32, gate_rows dividing rows (row r uses vector r / (rows / gate_rows)).
+ * residual may be null (the term is left out).  y is computed from the fp32 x_new: each output is rounded once.
+ * h, residual, x_new have leading dimensions ldh, ldr, ldx (elements, multiples of 8); y is contiguous.  x_new may be
+ * h or residual itself (same leading dimension), y may be h; x_new and y are different memory. */
+int samb_block_norm(const void* h, int64_t ldh, const void* residual, int64_t ldr, const float* post_gamma,
+                    const float* post_beta, const float* pre_gamma, const float* pre_beta, const float* gate,
+                    int64_t gate_rows, float res_scale, float eps, int is_f16, int rms, void* x_new, int64_t ldx, void* y,
+                    int64_t rows, int C, void* stream);
+
+/* The same (bf16) with y leaving as per-row symmetric int8 of the bf16-rounded norm, as samb_layernorm_quant_i8 gives
+ * it: yq [rows, C], y_scale [rows] = max(absmax, 1e-5) / 127. */
+int samb_block_norm_quant_i8(const void* h, int64_t ldh, const void* residual, int64_t ldr, const float* post_gamma,
+                             const float* post_beta, const float* pre_gamma, const float* pre_beta, const float* gate,
+                             int64_t gate_rows, float res_scale, float eps, int rms, void* x_new, int64_t ldx, int8_t* yq,
+                             float* y_scale, int64_t rows, int C, void* stream);
+
+/* Rotary positions on planes of rows: x[planes][rows][d] with plane_stride and row_stride in elements (multiples of
+ * 8; the q and k planes of samb_gemm_*_heads' output, or a [rows, heads, d] view with the two strides exchanged).
+ * Pair p < rot / 2 of a row, (a, b), becomes (a cos t - b sin t, b cos t + a sin t) * mscale with
+ * t = position * freqs[p]; the pairs are (2p, 2p + 1) when interleaved != 0, else (p, p + rot / 2); elements from rot
+ * on are copied.  positions[period][axes] is int32, or int64 when positions_i64 != 0: row r uses entry r % period
+ * (rows % period == 0).  With axes == 2 (rot % 4 == 0) the first half of the pairs turns with the first coordinate and
+ * the second half with the second.  freqs: DEVICE array of rot / 2 doubles, radians a position.  The angle
+ * is off by at most (2^-32 + |position| * 2^-63) turns.  out may be x itself with the same strides (in place). */
+int samb_rotary(const void* x, int64_t plane_stride, int64_t row_stride, const void* positions, int positions_i64,
+                int64_t period, int axes, const double* freqs, int rot, int interleaved, float mscale, void* out,
+                int64_t out_plane_stride, int64_t out_row_stride, int64_t planes, int64_t rows, int d, int is_f16,
+                void* stream);
+
+/* The router of a mixture of experts over logits[T, E] (fp32, leading dimension ld; E <= 512, k <= 8, k <= E):
+ *   ids[T, k]      experts of the k largest logits (+ bias[e], when given: it decides the choice only), largest first,
+ *                  ties to the lower index; -inf and NaN are never chosen, -1 stands where nobody is left
+ *   weights[T, k]  softmax over the row's logits (or their sigmoid when sigmoid != 0) at the chosen experts, divided
+ *                  by their sum when renorm != 0, times scale; 0 where ids is -1.  +inf counts as the largest float.
+ *   slots[T, k]    place of each (token, choice) in the order by expert (stable: by expert, then token, then choice), or -1
+ *   rows[T * k]    the token in each place, -1 behind the last
+ *   offsets[E + 1] first place of each expert, and their number
+ * scratch: samb_route_scratch_bytes(T, E) bytes (may be 0), 4-byte aligned, any contents; calls that may overlap on
+ * the GPU need one each. */
+int64_t samb_route_scratch_bytes(int64_t T, int E);
+int samb_route_topk(const float* logits, int64_t ld, const float* bias, int64_t T, int E, int k, int sigmoid, int renorm,
+                    float scale, int32_t* ids, float* weights, int32_t* slots, int32_t* rows, int32_t* offsets,
+                    void* scratch, void* stream);
+
+/* Products grouped by expert with ragged sizes: for offsets[e] <= s < offsets[e + 1]
+ *   out[s, :] = epilogue(A[rows ? rows[s] : s, :] * W[e]^T)
+ * A[a_rows, K], W[E][N, K] (leading dimension ldw, experts w_stride elements apart), out[S, N], all 16-bit with
+ * 16-byte aligned rows, N and K multiples of 8, E <= 512.  offsets[E + 1] is read on the device: values outside [0, S]
+ * are clamped, and an expert whose range falls back behind an earlier one's is empty.  Rows of out outside every range
+ * are left as they were.  rows (may be null; then a_rows >= S): an index outside [0, a_rows) stands for a row of
+ * zeros.  epilogue: SAMB_EPI_BIAS (bias fp32 [E, N]) and / or SAMB_EPI_GELU. */
+int samb_gemm_grouped(const void* A, int64_t lda, int64_t a_rows, const int32_t* rows, const void* W, int64_t ldw,
+                      int64_t w_stride, const float* bias, const int32_t* offsets, void* out, int64_t ldo, int64_t S,
+                      int E, int N, int K, int is_f16, int epilogue, int32_t* status, void* stream);
+/* The same on int8 operands (exact int32 accumulation; K % 16 == 0): the product is scaled by a_scale[row of A] and
+ * w_scale[e, n] before the epilogue; out is bf16. */
+int samb_gemm_i8_grouped(const int8_t* Aq, int64_t lda, int64_t a_rows, const float* a_scale, const int32_t* rows,
+                         const int8_t* Wq, int64_t ldw, int64_t w_stride, const float* w_scale, const float* bias,
+                         const int32_t* offsets, void* out, int64_t ldo, int64_t S, int E, int N, int K, int epilogue,
+                         int32_t* status, void* stream);
+
+/* Combination of the experts' rows: out[t, :] = residual[t, :] + sum_j weights[t, j] * x[slots[t, j], :], summed in
+ * fp32 in the order of j.  x[x_rows, C], residual (may be null) and out [T, C], C % 8 == 0, k <= 8.  A slot outside
+ * [0, x_rows) adds nothing.  out may be the residual itself (same leading dimension), not x. */
+int samb_combine_topk(const void* x, int64_t ldx, int64_t x_rows, const int32_t* slots, const float* weights,
+                      const void* residual, int64_t ldr, void* out, int64_t ldo, int64_t T, int k, int C, int is_f16,
+                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif

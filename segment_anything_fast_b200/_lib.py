@@ -58,6 +58,19 @@ SIGNATURES = {
     "samb_attn_relpos_window_tables": (c_int, [_P, _P, _P, _P, c_int64, c_int, c_int, c_int, c_int, c_int, c_float, _P, _P]),
     "samb_mask_stats": (c_int, [_P, c_int, c_int64, c_int, c_int, c_float, c_float, _P, _P, _P, _P, _P]),
     "samb_mask_rle": (c_int, [_P, c_int64, c_int, c_int, _P, _P, c_int, _P]),
+    "samb_block_norm": (c_int, [_P, c_int64, _P, c_int64, _P, _P, _P, _P, _P, c_int64, c_float, c_float, c_int, c_int, _P,
+                                c_int64, _P, c_int64, c_int, _P]),
+    "samb_block_norm_quant_i8": (c_int, [_P, c_int64, _P, c_int64, _P, _P, _P, _P, _P, c_int64, c_float, c_float, c_int, _P,
+                                         c_int64, _P, _P, c_int64, c_int, _P]),
+    "samb_rotary": (c_int, [_P, c_int64, c_int64, _P, c_int, c_int64, c_int, _P, c_int, c_int, c_float, _P, c_int64, c_int64,
+                            c_int64, c_int64, c_int, c_int, _P]),
+    "samb_route_scratch_bytes": (c_int64, [c_int64, c_int]),
+    "samb_route_topk": (c_int, [_P, c_int64, _P, c_int64, c_int, c_int, c_int, c_int, c_float, _P, _P, _P, _P, _P, _P, _P]),
+    "samb_gemm_grouped": (c_int, [_P, c_int64, c_int64, _P, _P, c_int64, c_int64, _P, _P, _P, c_int64, c_int64, c_int, c_int,
+                                  c_int, c_int, c_int, _P, _P]),
+    "samb_gemm_i8_grouped": (c_int, [_P, c_int64, c_int64, _P, _P, _P, c_int64, c_int64, _P, _P, _P, _P, c_int64, c_int64,
+                                     c_int, c_int, c_int, c_int, _P, _P]),
+    "samb_combine_topk": (c_int, [_P, c_int64, c_int64, _P, _P, _P, c_int64, _P, c_int64, c_int64, c_int, c_int, c_int, _P]),
     "samb_sp24_meta_bytes": (c_int64, [c_int, c_int]),
     "samb_pack_sp24": (c_int, [_P, c_int64, c_int, c_int, _P, c_int64, _P, _P, _P]),
     "samb_gemm_i8_sp24": (c_int, [_P, c_int64, _P, _P, c_int64, _P, _P, _P, _P, c_int64, c_int64, _P, c_int64,

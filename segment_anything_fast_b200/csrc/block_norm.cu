@@ -1,0 +1,304 @@
+// The norms on either side of a residual addition in one pass over the rows:
+//   x' = res_scale * r + gate * post(h),   y = pre(x'),
+// post and pre being LayerNorm or root-mean-square norms (or absent), gate one vector for all rows or one for each
+// of G equal blocks of rows (images).  y is computed from the fp32 x', not from its rounded copy: x' and y are each
+// rounded once.
+//
+// A thread owns eight fixed columns and walks down the rows, kRows of them at a time, so the affine parameters and
+// the gate (20 bytes a column against the 8 bytes a column that a row moves) stay in its registers.  A block is as
+// many warps as the width needs.  Statistics: a warp reduces its own 256 columns in two passes (mean, then squared
+// distances from it), and the warps' pairs (mean, M2) are joined by the parallel-variance formula
+//   M2 = sum_w M2_w + n_w (mean_w - mean)^2,
+// so a norm costs one block barrier for kRows rows and no difference of large squares is ever taken.
+#include "elem16.cuh"
+
+namespace samb {
+namespace {
+
+struct NormParams {
+  const void* h;
+  const void* r;
+  const float* post_g;
+  const float* post_b;
+  const float* pre_g;
+  const float* pre_b;
+  const float* gate;
+  void* x;
+  void* y;               // 16-bit rows, or int8 rows when quantising
+  float* y_scale;
+  long long ldh, ldr, ldx;
+  int rows, C, rows_per_gate, rows_per_block;
+  float res_scale, eps;
+};
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+__device__ __forceinline__ void load8(const float* p, int c, float (&v)[8]) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p + c)), b = __ldg(reinterpret_cast<const float4*>(p + c) + 1);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void fill8(float (&v)[8], float x) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = x;
+}
+
+// Statistics of kRows rows whose columns are spread over the block: on return sub[i] is what to subtract and
+// mul[i] what to multiply by.  `stat` is shared scratch for kRows * warps pairs; a caller alternates between two of
+// them, so that a buffer's next writes are a barrier away from its last reads.
+template <bool kRms, int kRows>
+__device__ __forceinline__ void row_stats(const float (&v)[kRows][8], bool live, int C, float eps, float2* stat,
+                                          float (&sub)[kRows], float (&mul)[kRows]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const float inv_n = 1.0f / float(min(256, C - warp * 256));      // columns of this warp
+  float2 mine[kRows];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    float mean = 0.f, m2 = 0.f;
+    if (!kRms) {
+      float s = 0.f;
+      if (live) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += v[i][j];
+      }
+      mean = warp_sum(s) * inv_n;
+    }
+    if (live) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float d = v[i][j] - mean;
+        m2 = fmaf(d, d, m2);
+      }
+    }
+    mine[i] = make_float2(mean, warp_sum(m2));
+  }
+  if (warps > 1) {
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) stat[warp * kRows + i] = mine[i];
+    }
+    __syncthreads();
+  }
+  const float inv_c = 1.0f / float(C);
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    float mean = mine[i].x, m2 = mine[i].y;
+    if (warps > 1) {
+      mean = 0.f;
+      if (!kRms) {                                       // around the first warp's: a constant row stays exact
+        const float first = stat[i].x;
+        for (int w = 1; w < warps; ++w) mean = fmaf(stat[w * kRows + i].x - first, float(min(256, C - w * 256)), mean);
+        mean = fmaf(mean, inv_c, first);
+      }
+      m2 = 0.f;
+      for (int w = 0; w < warps; ++w) {
+        const float2 s = stat[w * kRows + i];
+        const float d = s.x - mean;
+        m2 += s.y;
+        if (!kRms) m2 = fmaf(d * d, float(min(256, C - w * 256)), m2);
+      }
+    }
+    sub[i] = mean;
+    mul[i] = rsqrtf(fmaf(m2, inv_c, eps));
+  }
+}
+
+// kWide: up to 32 warps a block (C up to 8192), which leaves 64 registers a thread: the parameters are then read
+// where they are used.
+template <typename T, bool kRms, bool kQuant, int kRows, bool kWide>
+__global__ void __launch_bounds__(kWide ? 1024 : 256)
+block_norm_kernel(const NormParams p) {
+  constexpr int kPairs = kRows * (kWide ? 32 : 8);
+  __shared__ float2 s_post[2][kPairs], s_pre[2][kPairs];
+  __shared__ float s_max[kPairs];            // used between the barriers of two norms
+  int turn = 0;
+  const int c = int(threadIdx.x) * 8;
+  const bool live = c < p.C;
+  const int begin = int(blockIdx.x) * p.rows_per_block;
+  const int end = min(p.rows, begin + p.rows_per_block);
+  const bool has_post = p.post_g != nullptr, has_pre = p.pre_g != nullptr;
+
+  float pg[8], pb[8], qg[8], qb[8];          // post's gain and offset (times the gate), pre's gain and offset
+  fill8(pg, 1.f); fill8(pb, 0.f); fill8(qg, 1.f); fill8(qb, 0.f);
+  auto load_post = [&](int row) {
+    fill8(pg, 1.f);
+    fill8(pb, 0.f);
+    if (!live) return;
+    if (has_post) load8(p.post_g, c, pg);
+    if (p.post_b != nullptr) load8(p.post_b, c, pb);
+    if (p.gate != nullptr) {
+      float g[8];
+      load8(p.gate + (long long)(row / p.rows_per_gate) * p.C, c, g);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        pg[j] *= g[j];
+        pb[j] *= g[j];
+      }
+    }
+  };
+  auto load_pre = [&]() {
+    if (!live) return;
+    if (has_pre) load8(p.pre_g, c, qg);
+    if (p.pre_b != nullptr) load8(p.pre_b, c, qb);
+  };
+  int next_gate = begin;                     // first row that needs another gate vector than the one held
+  if (!kWide) load_pre();
+
+  for (int row0 = begin; row0 < end; row0 += kRows, turn ^= 1) {
+    uint4 hr[kRows], rr[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      hr[i] = rr[i] = make_uint4(0u, 0u, 0u, 0u);
+      const int row = row0 + i;
+      if (live && row < end) {
+        hr[i] = *(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.h) + row * p.ldh + c));
+        if (p.r != nullptr) rr[i] = *(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.r) + row * p.ldr + c));
+      }
+    }
+    float v[kRows][8], sub[kRows], mul[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) T::unpack(hr[i], v[i]);
+    if (has_post) {
+      row_stats<kRms, kRows>(v, live, p.C, p.eps, s_post[turn], sub, mul);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) { sub[i] = 0.f; mul[i] = 1.f; }
+    }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const int row = row0 + i;
+      if (row < end && (kWide || row >= next_gate)) {                // the same for every thread
+        load_post(row);
+        next_gate = (row / p.rows_per_gate + 1) * p.rows_per_gate;   // <= rows: whole blocks of rows
+      }
+      float r[8];
+      T::unpack(rr[i], r);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = fmaf((v[i][j] - sub[i]) * mul[i], pg[j], fmaf(p.res_scale, r[j], pb[j]));
+      if (live && row < end)
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.x) + row * p.ldx + c) = T::pack(v[i]);
+    }
+    if (!has_pre) continue;
+    row_stats<kRms, kRows>(v, live, p.C, p.eps, s_pre[turn], sub, mul);
+    if (kWide) load_pre();
+    uint4 out[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = fmaf((v[i][j] - sub[i]) * mul[i], qg[j], qb[j]);
+      out[i] = T::pack(f);
+      if (!kQuant && live && row0 + i < end)
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.y) + (long long)(row0 + i) * p.C + c) = out[i];
+    }
+    if (kQuant) {
+      // the rounded row, as a quantised Linear fed with 16-bit rows would see it
+      const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+      float amax[kRows];
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const float m = live ? absmax_fold(absmax8(__floats2bfloat162_rn(0.f, 0.f), out[i])) : 0.f;
+        amax[i] = warp_max(m);
+        if (warps > 1 && lane == 0) s_max[warp * kRows + i] = amax[i];
+      }
+      if (warps > 1) __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        for (int w = 0; warps > 1 && w < warps; ++w) amax[i] = fmaxf(amax[i], s_max[w * kRows + i]);
+        float sc, inv_sc;
+        row_scale(amax[i], sc, inv_sc);
+        if (row0 + i < end) {
+          if (threadIdx.x == 0) p.y_scale[row0 + i] = sc;
+          if (live)
+            *reinterpret_cast<uint2*>(static_cast<int8_t*>(p.y) + (long long)(row0 + i) * p.C + c) = quant8(out[i], sc, inv_sc);
+        }
+      }
+    }
+  }
+}
+
+template <typename T, bool kRms, bool kQuant>
+int launch_typed(NormParams& p, cudaStream_t st) {
+  const int warps = (p.C + 255) / 256;
+  const bool wide = warps > 8;
+  const int per_sm = wide ? 1 : 2048 / (warps * 32) < 4 ? 2048 / (warps * 32) : 4;
+  const long long slots = (long long)sm_count() * per_sm;
+  long long per_block = (p.rows + slots - 1) / slots;
+  if (!wide && per_block >= 4) {
+    per_block = (per_block + 3) / 4 * 4;
+    p.rows_per_block = int(per_block);
+    const unsigned blocks = unsigned((p.rows + per_block - 1) / per_block);
+    block_norm_kernel<T, kRms, kQuant, 4, false><<<blocks, warps * 32, 0, st>>>(p);
+  } else {
+    p.rows_per_block = int(per_block);
+    const unsigned blocks = unsigned((p.rows + per_block - 1) / per_block);
+    if (wide) block_norm_kernel<T, kRms, kQuant, 1, true><<<blocks, warps * 32, 0, st>>>(p);
+    else block_norm_kernel<T, kRms, kQuant, 1, false><<<blocks, warps * 32, 0, st>>>(p);
+  }
+  return launch_status();
+}
+
+int launch_block_norm(const void* h, int64_t ldh, const void* r, int64_t ldr, const float* post_g, const float* post_b,
+                      const float* pre_g, const float* pre_b, const float* gate, int64_t gate_rows, float res_scale,
+                      float eps, int is_f16, int rms, void* x, int64_t ldx, void* y, float* y_scale, bool quant,
+                      int64_t rows, int C, void* stream) {
+  if (rows < 0 || C <= 0 || (rows > 0 && (h == nullptr || x == nullptr))) return SAMB_E_BADARG;
+  if ((post_g == nullptr && post_b != nullptr) || (pre_g == nullptr && pre_b != nullptr)) return SAMB_E_BADARG;
+  if (rows > 0 && ((pre_g == nullptr) != (y == nullptr) || (quant && (y == nullptr || y_scale == nullptr)))) return SAMB_E_BADARG;
+  // outputs over inputs: row by row in place, so the rows have to lie alike
+  if ((x != nullptr && (x == y || (x == h && ldx != ldh) || (x == r && ldx != ldr))) ||
+      (y != nullptr && ((y == h && (quant || ldh != C)) || (y == r && (quant || ldr != C)))))
+    return SAMB_E_BADARG;
+  if (gate != nullptr && (gate_rows <= 0 || rows % gate_rows)) return SAMB_E_SHAPE;
+  if (C % 8 || C > 8192 || rows >= (int64_t(1) << 31)) return SAMB_E_SHAPE;
+  if (ldh % 8 || ldx % 8 || ldh < C || ldx < C || (r != nullptr && (ldr % 8 || ldr < C))) return SAMB_E_SHAPE;
+  const uintptr_t mis = reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(r) | reinterpret_cast<uintptr_t>(x) |
+                        reinterpret_cast<uintptr_t>(post_g) | reinterpret_cast<uintptr_t>(post_b) |
+                        reinterpret_cast<uintptr_t>(pre_g) | reinterpret_cast<uintptr_t>(pre_b) |
+                        reinterpret_cast<uintptr_t>(gate) | reinterpret_cast<uintptr_t>(y);
+  if (mis & 15u) return SAMB_E_ALIGN;
+  if (int e = check_device_arch()) return e;
+  if (rows == 0) return SAMB_OK;
+  NormParams p;
+  p.h = h; p.r = r; p.post_g = post_g; p.post_b = post_b; p.pre_g = pre_g; p.pre_b = pre_b; p.gate = gate;
+  p.x = x; p.y = y; p.y_scale = y_scale;
+  p.ldh = ldh; p.ldr = ldr; p.ldx = ldx;
+  p.rows = int(rows); p.C = C;
+  p.rows_per_gate = int(gate != nullptr ? rows / gate_rows : rows);
+  p.res_scale = res_scale; p.eps = eps;
+  auto st = static_cast<cudaStream_t>(stream);
+  if (quant) return rms ? launch_typed<Bf16, true, true>(p, st) : launch_typed<Bf16, false, true>(p, st);
+  if (is_f16) return rms ? launch_typed<F16, true, false>(p, st) : launch_typed<F16, false, false>(p, st);
+  return rms ? launch_typed<Bf16, true, false>(p, st) : launch_typed<Bf16, false, false>(p, st);
+}
+
+}  // namespace
+}  // namespace samb
+
+extern "C" {
+
+int samb_block_norm(const void* h, int64_t ldh, const void* residual, int64_t ldr, const float* post_gamma,
+                    const float* post_beta, const float* pre_gamma, const float* pre_beta, const float* gate,
+                    int64_t gate_rows, float res_scale, float eps, int is_f16, int rms, void* x_new, int64_t ldx, void* y,
+                    int64_t rows, int C, void* stream) {
+  return samb::launch_block_norm(h, ldh, residual, ldr, post_gamma, post_beta, pre_gamma, pre_beta, gate, gate_rows,
+                                 res_scale, eps, is_f16, rms, x_new, ldx, y, nullptr, false, rows, C, stream);
+}
+
+int samb_block_norm_quant_i8(const void* h, int64_t ldh, const void* residual, int64_t ldr, const float* post_gamma,
+                             const float* post_beta, const float* pre_gamma, const float* pre_beta, const float* gate,
+                             int64_t gate_rows, float res_scale, float eps, int rms, void* x_new, int64_t ldx, int8_t* yq,
+                             float* y_scale, int64_t rows, int C, void* stream) {
+  return samb::launch_block_norm(h, ldh, residual, ldr, post_gamma, post_beta, pre_gamma, pre_beta, gate, gate_rows,
+                                 res_scale, eps, 0, rms, x_new, ldx, yq, y_scale, true, rows, C, stream);
+}
+
+}  // extern "C"

@@ -2,7 +2,8 @@
 library owns every kernel.  Each wrapper validates dtype/device/contiguity,
 passes raw pointers plus the current CUDA stream, and raises on any error code.
 """
-from typing import Optional, Tuple
+import math
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -534,4 +535,288 @@ def normalize_u8(x: torch.Tensor, mean, std, out: Optional[torch.Tensor] = None)
     m = (ctypes.c_float * 3)(*[float(v) for v in mean])
     s = (ctypes.c_float * 3)(*[float(v) for v in std])
     _lib.check(_lib.load().samb_normalize_u8(x.data_ptr(), out.data_ptr(), B, C, H, W, m, s, _stream()), "samb_normalize_u8")
+    return out
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# Operators of transformer blocks beside the reference's own kind: norms around a block, rotary positions, a mixture
+# of experts.  16-bit tensors are bfloat16 or float16.
+# ---------------------------------------------------------------------------------------------------------------
+_HALF = (torch.bfloat16, torch.float16)
+
+
+def _need16(t: torch.Tensor, name: str) -> None:
+    if t.dtype not in _HALF:
+        raise RuntimeError(f"{name}: expected bfloat16 or float16, got {t.dtype}")
+    _need(t, t.dtype, name)
+
+
+def _vector(t: Optional[torch.Tensor], name: str, *shape: int) -> Optional[int]:
+    """Pointer of a contiguous fp32 tensor of this shape (or None)."""
+    if t is None:
+        return None
+    _need(t, torch.float32, name)
+    if tuple(t.shape) != shape or not t.is_contiguous():
+        raise RuntimeError(f"{name}: expected a contiguous float32 tensor of shape {list(shape)}, got {list(t.shape)}")
+    return t.data_ptr()
+
+
+def _indexes(t: torch.Tensor, name: str, n: int) -> int:
+    _need(t, torch.int32, name)
+    if t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise RuntimeError(f"{name}: expected a contiguous int32 tensor of {n} elements, got {list(t.shape)}")
+    return t.data_ptr()
+
+
+def _matrix(t: torch.Tensor, name: str) -> int:
+    """Leading dimension of a row-major matrix; a single row has none of its own."""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise RuntimeError(f"{name}: expected a 2-D tensor with unit inner stride")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _block_norm_args(h, residual, post, pre, gate, out):
+    _need16(h, "h")
+    ldh = _matrix(h, "h")
+    rows, C = h.shape
+    ldr = 0
+    if residual is not None:
+        _need(residual, h.dtype, "residual")
+        ldr = _matrix(residual, "residual")
+        if residual.shape != h.shape:
+            raise RuntimeError("residual must have the shape of h")
+    if out is None:
+        out = torch.empty(rows, C, dtype=h.dtype, device=h.device)
+    else:
+        _need(out, h.dtype, "out")
+        if out.shape != h.shape:
+            raise RuntimeError("out must have the shape of h")
+    post_g, post_b = post if post is not None else (None, None)
+    pre_g, pre_b = pre if pre is not None else (None, None)
+    gate_rows = 0
+    if gate is not None:
+        gate_rows = gate.shape[0] if gate.dim() == 2 else 1
+        if gate_rows == 0 or rows % gate_rows:
+            raise RuntimeError(f"gate: {gate_rows} vectors do not divide {rows} rows")
+    args = (h.data_ptr(), ldh, _ptr(residual), ldr, _vector(post_g, "post gain", C), _vector(post_b, "post offset", C),
+            _vector(pre_g, "pre gain", C), _vector(pre_b, "pre offset", C),
+            _vector(gate, "gate", *((gate_rows, C) if gate is not None and gate.dim() == 2 else (C,))), gate_rows)
+    return args, out, _matrix(out, "out"), rows, C
+
+
+def block_norm(h: torch.Tensor, residual: Optional[torch.Tensor] = None, post=None, pre=None,
+               gate: Optional[torch.Tensor] = None, res_scale: float = 1.0, eps: float = 1e-6, rms: bool = False,
+               out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """The norms before and after a residual addition in one pass: ``x = res_scale * residual + gate * post(h)`` and
+    ``y = pre(x)`` over rows ``[rows, C]`` (C a multiple of 8 up to 8192); returns ``(x, y)``, y being None without
+    ``pre``.  ``post`` / ``pre`` are ``(gain, offset or None)`` in fp32, LayerNorm or with ``rms`` root-mean-square
+    norms; ``gate`` is fp32 ``[C]``, or ``[G, C]`` with one vector for each of G equal blocks of rows.  ``out`` (x) may
+    be ``residual`` or ``h``."""
+    args, out, ldx, rows, C = _block_norm_args(h, residual, post, pre, gate, out)
+    y = torch.empty(rows, C, dtype=h.dtype, device=h.device) if pre is not None else None
+    _lib.check(_lib.load().samb_block_norm(*args, res_scale, eps, h.dtype == torch.float16, rms, out.data_ptr(), ldx,
+                                           _ptr(y), rows, C, _stream()), "samb_block_norm")
+    return out, y
+
+
+def block_norm_quant_i8(h: torch.Tensor, residual: Optional[torch.Tensor], post, pre, gate: Optional[torch.Tensor] = None,
+                        res_scale: float = 1.0, eps: float = 1e-6, rms: bool = False,
+                        out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``block_norm`` (bf16) whose y leaves quantised per row for an int8 Linear: returns ``(x, yq, y_scale)``, the
+    values ``quant_rows_i8`` gives on y."""
+    _need(h, torch.bfloat16, "h")
+    if pre is None:
+        raise RuntimeError("block_norm_quant_i8 needs the norm whose output it quantises")
+    args, out, ldx, rows, C = _block_norm_args(h, residual, post, pre, gate, out)
+    yq = torch.empty(rows, C, dtype=torch.int8, device=h.device)
+    scale = torch.empty(rows, dtype=torch.float32, device=h.device)
+    _lib.check(_lib.load().samb_block_norm_quant_i8(*args, res_scale, eps, rms, out.data_ptr(), ldx, yq.data_ptr(),
+                                                    scale.data_ptr(), rows, C, _stream()), "samb_block_norm_quant_i8")
+    return out, yq, scale
+
+
+def rotary_freqs(rot: int, base: float = 10000.0, axes: int = 1, scaling: Optional[str] = None, factor: float = 1.0,
+                 trained: int = 4096, device=None) -> Tuple[torch.Tensor, float]:
+    """Angular frequencies (float64 ``[rot / 2]``, radians a position) and the factor on the rotation for ``rotary``:
+    ``base ** (-i / n)`` for the n pairs of each axis.  ``scaling`` stretches them by ``factor`` for positions beyond
+    the ``trained`` length: ``"linear"`` divides every frequency, ``"base"`` raises the base so that the slowest pair
+    is stretched by the factor and the fastest not at all, ``"parts"`` keeps pairs of more than 32 turns over the
+    trained length, divides those of less than one, ramps in between and scales the rotation by
+    ``0.1 ln(factor) + 1`` (the YaRN rule)."""
+    if rot <= 0 or axes not in (1, 2) or rot % (2 * axes):
+        raise RuntimeError(f"rotary_freqs: {rot} rotated elements do not make pairs on {axes} axes")
+    if scaling not in (None, "linear", "base", "parts"):
+        raise RuntimeError(f"rotary_freqs: unknown scaling {scaling!r}")
+    if not (base > 0 and factor >= 1 and trained > 0):
+        raise RuntimeError("rotary_freqs: base and trained must be positive and factor at least 1")
+    n = rot // 2 // axes
+    i = torch.arange(n, dtype=torch.float64)
+    if scaling == "base" and n > 1:
+        base = base * factor ** (n / (n - 1))
+    f = base ** (-i / n)
+    mscale = 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "parts":
+        keep = ((trained * f / (2 * math.pi) - 1.0) / 31.0).clamp(0.0, 1.0)
+        f = f * (keep + (1.0 - keep) / factor)
+        mscale = 0.1 * math.log(factor) + 1.0
+    return f.repeat(axes).to(device or torch.device("cuda", torch.cuda.current_device())), mscale
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, interleaved: bool = False,
+           mscale: float = 1.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotary positions on ``x [planes, rows, d]`` (any plane and row strides that are multiples of 8: the q and k planes
+    ``qkv[:2 * H]`` of ``gemm_heads``, or a ``[rows, heads, d]`` tensor seen as ``x.transpose(0, 1)``).  Pairs are
+    neighbours (``interleaved``) or half the rotated width apart; the first ``2 * len(freqs)`` elements of a row turn,
+    the rest is copied.  ``positions`` int32 / int64: ``[P]``, or ``[P, 2]`` for a raster (first half of the pairs by the
+    first coordinate); row r uses entry ``r % P``.  ``freqs`` float64, see ``rotary_freqs``.  ``out`` may be ``x``."""
+    _need16(x, "x")
+    _need(freqs, torch.float64, "freqs")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError(f"positions: expected int32 or int64, got {positions.dtype}")
+    _need(positions, positions.dtype, "positions")
+    if x.dim() != 3 or (x.shape[2] > 1 and x.stride(2) != 1):
+        raise RuntimeError("x: expected a [planes, rows, d] tensor with unit inner stride")
+    planes, rows, d = x.shape
+    if positions.dim() not in (1, 2) or not positions.is_contiguous() or (positions.dim() == 2 and positions.shape[1] != 2):
+        raise RuntimeError("positions: expected a contiguous [P] or [P, 2] tensor")
+    period, axes = positions.shape[0], positions.dim()
+    if rows and (period == 0 or rows % period):
+        raise RuntimeError(f"positions: {period} entries do not divide {rows} rows")
+    if freqs.dim() != 1 or not freqs.is_contiguous():
+        raise RuntimeError("freqs: expected a contiguous 1-D tensor")
+    if out is None:
+        out = torch.empty(planes, rows, d, dtype=x.dtype, device=x.device)
+    elif out is not x:
+        _need(out, x.dtype, "out")
+        if out.shape != x.shape or (d > 1 and out.stride(2) != 1):
+            raise RuntimeError("out must have the shape of x and unit inner stride")
+    _lib.check(_lib.load().samb_rotary(
+        x.data_ptr(), x.stride(0) if planes > 1 else 0, x.stride(1) if rows > 1 else 0, positions.data_ptr(),
+        positions.dtype == torch.int64, period, axes, freqs.data_ptr(), 2 * freqs.shape[0], interleaved, mscale,
+        out.data_ptr(), out.stride(0) if planes > 1 else 0, out.stride(1) if rows > 1 else 0, planes, rows, d,
+        x.dtype == torch.float16, _stream()), "samb_rotary")
+    return out
+
+
+class Routing(NamedTuple):
+    """What ``route_topk`` found: ``ids`` and ``weights`` ``[T, k]``, ``slots [T, k]`` (place of each choice in the order
+    by expert, -1: none), ``rows [T * k]`` (token in each place, -1 behind the last), ``offsets [E + 1]``."""
+    ids: torch.Tensor
+    weights: torch.Tensor
+    slots: torch.Tensor
+    rows: torch.Tensor
+    offsets: torch.Tensor
+
+
+def route_topk(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] = None, sigmoid: bool = False,
+               renorm: bool = True, scale: float = 1.0) -> Routing:
+    """Router of a mixture of experts over fp32 ``logits [T, E]`` (E up to 512, k up to 8): every token's k largest
+    logits (plus ``bias [E]``, which decides the choice only; ties to the lower index), their softmax or sigmoid
+    weights, and the order of the choices by expert for ``gemm_grouped`` and ``combine_topk``.  An expert at -inf or NaN
+    is never chosen: a token with nobody left (a padded one) gets id -1, weight 0 and no place."""
+    _need(logits, torch.float32, "logits")
+    ld = _matrix(logits, "logits")
+    T, E = logits.shape
+    if not 1 <= k <= min(8, E):
+        raise RuntimeError(f"k: {k} is not between 1 and 8 and at most the number of experts ({E})")
+    dev = logits.device
+    lib = _lib.load()
+    n = T * k
+    scratch = lib.samb_route_scratch_bytes(T, E) // 4
+    # one allocation for the whole numbers: ids, slots, rows, offsets, scratch
+    buf = torch.empty(3 * n + E + 1 + scratch, dtype=torch.int32, device=dev)
+    weights = torch.empty(T, k, dtype=torch.float32, device=dev)
+    at = buf.data_ptr()
+    _lib.check(lib.samb_route_topk(
+        logits.data_ptr(), ld, _vector(bias, "bias", E), T, E, k, sigmoid, renorm, scale, at, weights.data_ptr(),
+        at + 4 * n, at + 8 * n, at + 12 * n, at + 4 * (3 * n + E + 1), _stream()), "samb_route_topk")
+    return Routing(buf.as_strided((T, k), (k, 1), 0), weights, buf.as_strided((T, k), (k, 1), n),
+                   buf.as_strided((n,), (1,), 2 * n), buf.as_strided((E + 1,), (1,), 3 * n))
+
+
+def _grouped_args(a, w, offsets, rows, bias, out, out_dtype, kind):
+    lda = _matrix(a, "a")
+    if w.dim() != 3 or (w.shape[2] > 1 and w.stride(2) != 1):
+        raise RuntimeError("w: expected an [experts, N, K] tensor with unit inner stride")
+    E, N, K = w.shape
+    if a.shape[1] != K:
+        raise RuntimeError(f"{kind}: inner dimensions differ")
+    S = rows.shape[0] if rows is not None else a.shape[0]
+    if out is None:
+        out = torch.empty(S, N, dtype=out_dtype, device=a.device)
+    else:
+        _need(out, out_dtype, "out")
+        if out.shape != (S, N):
+            raise RuntimeError(f"out: expected [{S}, {N}], got {list(out.shape)}")
+    return (lda, _indexes(rows, "rows", S) if rows is not None else None, w.stride(1) if N > 1 else K,
+            w.stride(0) if E > 1 else 0, _vector(bias, "bias", E, N), _indexes(offsets, "offsets", E + 1), out,
+            _matrix(out, "out"), S, E, N, K)
+
+
+def gemm_grouped(a: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows: Optional[torch.Tensor] = None,
+                 bias: Optional[torch.Tensor] = None, gelu: bool = False,
+                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Products grouped by expert: ``out[s] = act(a[rows[s]] @ w[e]^T + bias[e])`` for ``offsets[e] <= s < offsets[e + 1]``
+    (without ``rows``: ``a[s]``), with ``a [M, K]`` and ``w [E, N, K]`` bfloat16 or float16, int32 ``offsets [E + 1]`` and
+    ``rows [S]`` as ``route_topk`` gives them.  Rows of ``out [S, N]`` behind the last expert's are left as they were
+    (unspecified in a new ``out``); an index outside ``a`` stands for a row of zeros."""
+    _need16(a, "a"); _need(w, a.dtype, "w")
+    lda, prow, ldw, ws, pbias, poff, out, ldo, S, E, N, K = _grouped_args(a, w, offsets, rows, bias, out, a.dtype,
+                                                                         "gemm_grouped")
+    _lib.check(_lib.load().samb_gemm_grouped(
+        a.data_ptr(), lda, a.shape[0], prow, w.data_ptr(), ldw, ws, pbias, poff, out.data_ptr(), ldo, S, E, N, K,
+        a.dtype == torch.float16, (EPI_BIAS if bias is not None else 0) | (EPI_GELU if gelu else 0),
+        status_word(a.device).data_ptr(), _stream()), "samb_gemm_grouped")
+    return out
+
+
+def gemm_i8_grouped(aq: torch.Tensor, a_scale: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor,
+                    offsets: torch.Tensor, rows: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                    gelu: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``gemm_grouped`` on int8 ``aq [M, K]`` with row scales ``a_scale [M]`` (gathered with the rows) and ``wq [E, N, K]``
+    with ``w_scale [E, N]``: exact int32 accumulation, bf16 out."""
+    _need(aq, torch.int8, "aq"); _need(wq, torch.int8, "wq")
+    lda, prow, ldw, ws, pbias, poff, out, ldo, S, E, N, K = _grouped_args(aq, wq, offsets, rows, bias, out,
+                                                                         torch.bfloat16, "gemm_i8_grouped")
+    if a_scale is None or w_scale is None:
+        raise RuntimeError("gemm_i8_grouped needs both scales")
+    _lib.check(_lib.load().samb_gemm_i8_grouped(
+        aq.data_ptr(), lda, aq.shape[0], _vector(a_scale, "a_scale", aq.shape[0]), prow, wq.data_ptr(), ldw, ws,
+        _vector(w_scale, "w_scale", E, N), pbias, poff, out.data_ptr(), ldo, S, E, N, K,
+        (EPI_BIAS if bias is not None else 0) | (EPI_GELU if gelu else 0), status_word(aq.device).data_ptr(),
+        _stream()), "samb_gemm_i8_grouped")
+    return out
+
+
+def combine_topk(x: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, residual: Optional[torch.Tensor] = None,
+                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Weighted sum of the experts' rows back in token order: ``out[t] = residual[t] + sum_j weights[t, j] *
+    x[slots[t, j]]`` with ``x [S, C]`` bfloat16 or float16, ``slots`` / ``weights`` ``[T, k]`` of ``route_topk`` (k up to 8);
+    a slot of -1 adds nothing.  ``out`` may be ``residual``."""
+    _need16(x, "x")
+    ldx = _matrix(x, "x")
+    S, C = x.shape
+    if slots.dim() != 2:
+        raise RuntimeError("slots: expected a [T, k] tensor")
+    T, k = slots.shape
+    _need(slots, torch.int32, "slots")
+    if not slots.is_contiguous():
+        raise RuntimeError("slots must be contiguous")
+    ldr = 0
+    if residual is not None:
+        _need(residual, x.dtype, "residual")
+        ldr = _matrix(residual, "residual")
+        if residual.shape != (T, C):
+            raise RuntimeError(f"residual: expected [{T}, {C}], got {list(residual.shape)}")
+    if out is None:
+        out = torch.empty(T, C, dtype=x.dtype, device=x.device)
+    else:
+        _need(out, x.dtype, "out")
+        if out.shape != (T, C):
+            raise RuntimeError(f"out: expected [{T}, {C}], got {list(out.shape)}")
+    _lib.check(_lib.load().samb_combine_topk(
+        x.data_ptr(), ldx, S, slots.data_ptr(), _vector(weights, "weights", T, k), _ptr(residual), ldr, out.data_ptr(),
+        _matrix(out, "out"), T, k, C, x.dtype == torch.float16, _stream()), "samb_combine_topk")
     return out
