@@ -394,16 +394,20 @@ int samb_route_topk(const float* logits, int64_t ld, const float* bias, int64_t 
  * 16-byte aligned rows, N and K multiples of 8, E <= 512.  offsets[E + 1] is read on the device: values outside [0, S]
  * are clamped, and an expert whose range falls back behind an earlier one's is empty.  Rows of out outside every range
  * are left as they were.  rows (may be null; then a_rows >= S): an index outside [0, a_rows) stands for a row of
- * zeros.  epilogue: SAMB_EPI_BIAS (bias fp32 [E, N]) and / or SAMB_EPI_GELU. */
+ * zeros.  epilogue: SAMB_EPI_BIAS (bias fp32 [E, N]) and / or SAMB_EPI_GELU.
+ * scratch: samb_gemm_grouped_scratch_bytes bytes (0 for few rows), 16-byte aligned, any contents, used with rows only:
+ * large products put the rows in order there first.  Null is allowed and slower.  Calls that may overlap on the GPU
+ * need one each. */
+int64_t samb_gemm_grouped_scratch_bytes(int64_t S, int E, int K, int is_i8);
 int samb_gemm_grouped(const void* A, int64_t lda, int64_t a_rows, const int32_t* rows, const void* W, int64_t ldw,
                       int64_t w_stride, const float* bias, const int32_t* offsets, void* out, int64_t ldo, int64_t S,
-                      int E, int N, int K, int is_f16, int epilogue, int32_t* status, void* stream);
+                      int E, int N, int K, int is_f16, int epilogue, void* scratch, int32_t* status, void* stream);
 /* The same on int8 operands (exact int32 accumulation; K % 16 == 0): the product is scaled by a_scale[row of A] and
  * w_scale[e, n] before the epilogue; out is bf16. */
 int samb_gemm_i8_grouped(const int8_t* Aq, int64_t lda, int64_t a_rows, const float* a_scale, const int32_t* rows,
                          const int8_t* Wq, int64_t ldw, int64_t w_stride, const float* w_scale, const float* bias,
                          const int32_t* offsets, void* out, int64_t ldo, int64_t S, int E, int N, int K, int epilogue,
-                         int32_t* status, void* stream);
+                         void* scratch, int32_t* status, void* stream);
 
 /* Combination of the experts' rows: out[t, :] = residual[t, :] + sum_j weights[t, j] * x[slots[t, j], :], summed in
  * fp32 in the order of j.  x[x_rows, C], residual (may be null) and out [T, C], C % 8 == 0, k <= 8.  A slot outside

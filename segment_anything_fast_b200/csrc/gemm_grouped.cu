@@ -1,16 +1,20 @@
 // Products grouped by expert with ragged sizes (a mixture of experts' Linear layers):
 //   out[s, :] = epilogue( a[rows ? rows[s] : s, :] * w[e]^T + bias[e] ),   offsets[e] <= s < offsets[e + 1].
 // The offsets live on the device (the router wrote them), so the host launches one wave of persistent CTAs and every
-// CTA works the tile list out for itself: the prefix over the experts of their 128-row tiles, times the column tiles.
+// CTA works the tile list out for itself: the prefix over the experts of their row tiles, times the column tiles.
 //
-// Tile loop: warp 0 streams 128-byte K slabs of A and W into a ring of 128B-swizzled stages (TMA; with `rows` the A
-// rows are gathered four at a time by tile::gather4, so no permuted copy of the activations exists), warp 1 issues
-// tcgen05.mma into one of two accumulators in tensor memory, warps 2..9 drain the other one.  A tile reads 128 rows
-// of A whatever its expert has left (rows of the next expert, discarded), but stores only its own: whole tiles
-// leave by TMA, the last tile of an expert row by row from the staging tile.
+// Two kernels.  On CTA pairs (256 x 256 tiles, cta_group::2, each CTA loads its 128 rows of A and half of W) for groups
+// of a few hundred rows and more; on single CTAs (128 x 256, 128 or 64) below, where the weights' bytes count and the
+// number of tiles is what spreads their stream over the SMs.
 //
-// Column tile: 256, 128 or 64 wide, picked by the CTAs themselves so that the last wave is not mostly empty (a handful
-// of tokens touches each expert's weights once, and the number of tiles is what spreads that stream over the SMs).
+// Operands: 128-byte K slabs in a ring of 128B-swizzled stages, W by TMA, and A too when its rows lie in order.  With
+// `rows` the single-CTA kernel has a warp per stage fetch them with 16-byte cp.async into the same swizzled places.  The
+// pair kernel would gather every row again for each of its column tiles, faster than cp.async delivers them (774 us
+// against 590 us for rows in order at 65536 x 5120 x 1280; TMA's own gather of four rows, at some 85 cycles an
+// instruction, took 2110 us), so its rows are put in order first, in caller scratch: a pass at copy bandwidth (30 us).
+//
+// A tile computes all its rows whatever its expert has left, but stores only its own: whole 128-row halves leave by
+// TMA, the last ones of an expert row by row.
 #include "elem16.cuh"
 
 namespace samb {
@@ -19,24 +23,17 @@ namespace {
 constexpr int BM = 128;
 constexpr int BN = 256;
 constexpr int SLAB_BYTES = 128;
-constexpr int STAGES = 4;
 constexpr int A_STAGE_BYTES = BM * SLAB_BYTES;
-constexpr int B_BOX_ROWS = 64;
-constexpr int B_BOX_BYTES = B_BOX_ROWS * SLAB_BYTES;
-constexpr int B_STAGE_BYTES = BN * SLAB_BYTES;
-constexpr int STAGE_BYTES = A_STAGE_BYTES + B_STAGE_BYTES;
 constexpr int NUM_ACC = 2;
 constexpr int TMEM_COLS = NUM_ACC * BN;
-constexpr int EPI_WARPS = 8;
-constexpr int NUM_THREADS = 64 + 32 * EPI_WARPS;
 constexpr int OUT_STAGE_BYTES = BM * 128;
 constexpr int kMaxExperts = 512;
-constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + OUT_STAGE_BYTES + 2 * BN * 4 + 2 * (kMaxExperts + 1) * 4 + 1024 + 256;
 
 enum { kTypeBf16 = 0, kTypeF16 = 1, kTypeI8 = 2 };
 
 struct GroupedParams {
   void* out;
+  const uint8_t* a;                // for the gathering warps
   const float* bias;               // [E, N] or null
   const float* a_scale;            // int8: per row of A
   const float* w_scale;            // int8: [E, N]
@@ -44,10 +41,124 @@ struct GroupedParams {
   const int* offsets;              // [E + 1]
   int* status;
   long long ldo, a_rows, S;
+  long long a_pitch;               // bytes between rows of A
   int E, N, K;
-  int k_slabs, last_ksteps;
-  int gelu;
+  int k_bytes, k_slabs, last_ksteps;
 };
+
+// The tile list, by one warp: first[e] = row tiles (of tile_rows) before expert e, start[e] = its first slot.  Offsets
+// are clamped to [0, S] and made to rise, so that no list can point outside the buffers.  Returns the row tiles.
+__device__ __forceinline__ int tile_list(const GroupedParams& p, int tile_rows, int* first, int* start) {
+  const int lane = threadIdx.x & 31;
+  int tiles = 0, at = 0;
+  for (int e0 = 0; e0 < p.E; e0 += 32) {
+    const int e = e0 + lane;
+    int lo = 0, hi = 0;
+    if (e < p.E) {
+      lo = min(max(__ldg(p.offsets + e), 0), int(p.S));
+      hi = min(max(__ldg(p.offsets + e + 1), 0), int(p.S));
+    }
+    int top = max(lo, hi);                               // largest offset up to this expert
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, top, o);
+      if (lane >= o) top = max(top, up);
+    }
+    top = max(top, at);
+    int below = __shfl_up_sync(0xffffffffu, top, 1);
+    if (lane == 0) below = e0 == 0 ? lo : at;
+    const int begin = max(lo, below), n = max(0, hi - begin);
+    const int mine = (n + tile_rows - 1) / tile_rows;
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    if (e < p.E) {
+      first[e] = tiles + sum - mine;
+      start[e] = begin;
+      if (e == p.E - 1) start[p.E] = begin + n;
+    }
+    tiles += __shfl_sync(0xffffffffu, sum, 31);
+    at = __shfl_sync(0xffffffffu, top, 31);
+  }
+  if (lane == 0) first[p.E] = tiles;
+  return tiles;
+}
+
+// Where a tile lies.  Tiles are numbered expert by expert, row tile by row tile, column tile by column tile; a role
+// walks its tiles in rising order, so the expert only ever moves forward.
+struct TileWalk {
+  const int* first;
+  const int* start;
+  int tiles_n, tile_rows, e, m0, rows, ntile;
+  __device__ __forceinline__ TileWalk(const int* f, const int* s, int tn, int tr)
+      : first(f), start(s), tiles_n(tn), tile_rows(tr), e(0), m0(0), rows(0), ntile(0) {}
+  __device__ __forceinline__ void at(int tile) {
+    const int mt = tile / tiles_n;
+    ntile = tile - mt * tiles_n;
+    while (first[e + 1] <= mt) ++e;
+    m0 = start[e] + (mt - first[e]) * tile_rows;
+    rows = min(tile_rows, start[e + 1] - m0);
+  }
+};
+
+// A gathering warp owns one stage of the ring: for every STAGES-th slab it waits until the stage is free, fetches 128
+// rows of A (from row `skip` of the tile) with 32 cp.async a lane, eight lanes a row, waits for them and passes the slab
+// on.  Rows and columns that do not exist are filled with zeros.  cp.async writes through the generic proxy and the
+// tensor core reads through the async one; the fence between the two waits for the thread's copies in flight, so a
+// thread with several slabs in flight would pay the whole memory latency for each of them.  Here the warps overlap.
+template <int STAGES, int kStageBytes, typename Arrive>
+__device__ __forceinline__ void gather_role(const GroupedParams& p, TileWalk w, uint8_t* smem, uint64_t* empty_bar,
+                                            volatile int* abort_flag, int stage, int skip, int tile0, int step, int num_tiles,
+                                            Arrive arrive) {
+  const int lane = threadIdx.x & 31;
+  const int unit = lane & 7, quarter = lane >> 3;
+  // row 4 j + quarter goes to its 128 bytes, the 16-byte units exchanged as the 128B swizzle wants it
+  const uint32_t dst_even = smem_u32(smem) + stage * kStageBytes + quarter * 128 + ((unit ^ quarter) << 4);
+  const uint32_t dst_odd = smem_u32(smem) + stage * kStageBytes + quarter * 128 + ((unit ^ (quarter + 4)) << 4);
+  uint32_t phase = 0;
+  int slab = stage;                                      // slab of the current tile that is this warp's next
+  for (int tile = tile0; tile < num_tiles; tile += step, slab -= p.k_slabs) {
+    if (slab >= p.k_slabs) continue;
+    w.at(tile);
+    int idx[4];                                          // rows 32 i + lane of the tile
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int m = skip + i * 32 + lane;
+      const int r = m < w.rows ? __ldg(p.rows + w.m0 + m) : -1;
+      idx[i] = r < p.a_rows ? r : -1;
+    }
+    for (; slab < p.k_slabs; slab += STAGES) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, 8))) return;
+      const int k0 = slab * SLAB_BYTES + unit * 16;
+      const bool inside = k0 < p.k_bytes;
+      const uint8_t* base = p.a + (inside ? k0 : 0);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const int r = __shfl_sync(0xffffffffu, idx[j >> 3], (j & 7) * 4 + quarter);
+        const bool there = inside && r >= 0;
+        const uint8_t* s = base + (there ? r : 0) * p.a_pitch;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(((j & 1) ? dst_odd : dst_even) + j * 512), "l"(s),
+                     "r"(there ? 16 : 0)
+                     : "memory");
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      asm volatile("fence.proxy.async;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) arrive(stage);
+      phase ^= 1u;
+    }
+  }
+}
+
+// A wait gave up somewhere: the producer sees its copies in flight home before the CTA ends.
+template <int STAGES>
+__device__ __forceinline__ void drain_copies(uint64_t* full_bar, uint32_t issued) {
+  for (uint32_t i = issued > STAGES ? issued - STAGES : 0u; i < issued; ++i)
+    for (uint32_t n = 0; n < 4096u && !mbar_try_wait(&full_bar[i % STAGES], (i / STAGES) & 1u); ++n) __nanosleep(64);
+}
 
 __device__ __forceinline__ bool epi_all(bool pred) {
   uint32_t r;
@@ -61,36 +172,20 @@ __device__ __forceinline__ bool epi_all(bool pred) {
 }
 __device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-// Four rows of a 2-D tensor into 4 x 128 consecutive bytes.
-__device__ __forceinline__ void tma_gather4(void* smem_dst, const CUtensorMap* m, uint64_t* bar, int x, const int4& r) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
-      ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(x), "r"(r.x), "r"(r.y),
-      "r"(r.z), "r"(r.w)
-      : "memory");
-}
+// ---------------------------------------------------------------------------------------------- single CTAs
+constexpr int ONE_STAGES = 4;
+constexpr int ONE_STAGE_BYTES = A_STAGE_BYTES + BN * SLAB_BYTES;
+constexpr int B_BOX_ROWS = 64;
+constexpr int B_BOX_BYTES = B_BOX_ROWS * SLAB_BYTES;
+constexpr int ONE_THREADS = 64 + 256;                    // producer, MMA, eight epilogue warps (and the gathering ones)
+constexpr int ONE_SMEM_BYTES = ONE_STAGES * ONE_STAGE_BYTES + OUT_STAGE_BYTES + 2 * BN * 4 + 2 * (kMaxExperts + 1) * 4 + 1024 + 256;
 
-// Where a tile lies.  Tiles are numbered expert by expert, row tile by row tile, column tile by column tile; a role
-// walks its tiles in rising order, so the expert only ever moves forward.
-struct TileWalk {
-  const int* first;                // [E + 1] row tiles before each expert
-  const int* start;                // [E + 1] first slot of each expert, clamped
-  int tiles_n, e, m0, rows, ntile;
-  __device__ __forceinline__ TileWalk(const int* f, const int* s, int tn) : first(f), start(s), tiles_n(tn), e(0), m0(0), rows(0), ntile(0) {}
-  __device__ __forceinline__ void at(int tile) {
-    const int mt = tile / tiles_n;
-    ntile = tile - mt * tiles_n;
-    while (first[e + 1] <= mt) ++e;
-    m0 = start[e] + (mt - first[e]) * BM;
-    rows = min(BM, start[e + 1] - m0);
-  }
-};
-
-template <int kType, bool kGelu>
-__global__ void __launch_bounds__(NUM_THREADS, 1)
-gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                    const __grid_constant__ CUtensorMap tmOut, const GroupedParams p) {
+template <int kType, bool kGelu, bool kGather>
+__global__ void __launch_bounds__(ONE_THREADS + (kGather ? 32 * ONE_STAGES : 0), 1)
+grouped_one_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                   const __grid_constant__ CUtensorMap tmOut, const GroupedParams p) {
   constexpr bool kInt8 = kType == kTypeI8;
+  constexpr int STAGES = ONE_STAGES, STAGE_BYTES = ONE_STAGE_BYTES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* stage_out = smem + STAGES * STAGE_BYTES;
@@ -112,15 +207,15 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full_bar[s], 1);
+      mbar_init(&full_bar[s], 1 + (kGather ? 1 : 0));
       mbar_init(&empty_bar[s], 1);
     }
     for (int a = 0; a < NUM_ACC; ++a) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], EPI_WARPS);
+      mbar_init(&acc_empty[a], 8);
     }
     fence_mbar_init();
-    tma_prefetch_desc(&tmA);
+    if (!kGather) tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
     tma_prefetch_desc(&tmOut);
   }
@@ -129,44 +224,9 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     tmem_relinquish();
   }
   if (warp == 2) {
-    // the tile list.  Offsets are clamped to [0, S] and made to rise, so that no list can point outside the buffers.
-    int tiles = 0, at = 0;
-    for (int e0 = 0; e0 < p.E; e0 += 32) {
-      const int e = e0 + lane;
-      int lo = 0, hi = 0;
-      if (e < p.E) {
-        lo = min(max(__ldg(p.offsets + e), 0), int(p.S));
-        hi = min(max(__ldg(p.offsets + e + 1), 0), int(p.S));
-      }
-      int top = max(lo, hi);                             // running maximum over the experts up to this one
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, top, o);
-        if (lane >= o) top = max(top, up);
-      }
-      top = max(top, at);
-      int below = __shfl_up_sync(0xffffffffu, top, 1);
-      if (lane == 0) below = at;
-      if (e0 == 0 && lane == 0) below = lo;
-      const int begin = max(lo, below), n = max(0, hi - begin);
-      const int mine = (n + BM - 1) / BM;
-      int sum = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += up;
-      }
-      if (e < p.E) {
-        s_first[e] = tiles + sum - mine;
-        s_start[e] = begin;
-        if (e == p.E - 1) s_start[p.E] = begin + n;
-      }
-      tiles += __shfl_sync(0xffffffffu, sum, 31);
-      at = __shfl_sync(0xffffffffu, top, 31);
-    }
+    const int tiles = tile_list(p, BM, s_first, s_start);
     if (lane == 0) {
-      s_first[p.E] = tiles;
-      // waves x (columns + what a tile costs beside its columns)
+      // column tile: waves x (columns + what a tile costs beside its columns), so that the last wave is not mostly empty
       int best = 0, bn = BN;
       for (int w = BN; w >= 64; w >>= 1) {
         const long long t = (long long)tiles * ((p.N + w - 1) / w);
@@ -184,7 +244,7 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   const int tiles_n = (p.N + bn - 1) / bn;
   const int num_tiles = s_first[p.E] * tiles_n;
   constexpr int slab_elems = kInt8 ? SLAB_BYTES : SLAB_BYTES / 2;
-  TileWalk w(s_first, s_start, tiles_n);
+  TileWalk w(s_first, s_start, tiles_n, BM);
   uint32_t issued = 0;                                   // slabs that the producer has sent for
 
   if (warp == 0) {
@@ -194,24 +254,14 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
       w.at(tile);
       const int n0 = w.ntile * bn;
-      int4 src = make_int4(0, 0, 0, 0);                  // the four rows of A that this lane gathers
-      if (p.rows != nullptr) {
-        int r[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int m = lane * 4 + j;
-          const int i = m < w.rows ? __ldg(p.rows + w.m0 + m) : 0;
-          r[j] = i >= 0 && i < p.a_rows ? i : 0;         // outside A: any row, the epilogue drops its product
-        }
-        src = make_int4(r[0], r[1], r[2], r[3]);
-      }
       for (int ks = 0; ks < p.k_slabs; ++ks) {
         if (!(ok = __all_sync(0xffffffffu, mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, 1)))) break;
         uint8_t* sa = smem + stage * STAGE_BYTES;
-        if (lane == 0) mbar_expect_tx(&full_bar[stage], A_STAGE_BYTES + bn * SLAB_BYTES);
+        if (lane == 0) {
+          mbar_expect_tx(&full_bar[stage], (kGather ? 0 : A_STAGE_BYTES) + bn * SLAB_BYTES);
+          if (!kGather) tma_load_2d(sa, &tmA, &full_bar[stage], ks * slab_elems, w.m0);
+        }
         __syncwarp();
-        if (p.rows != nullptr) tma_gather4(sa + lane * 512, &tmA, &full_bar[stage], ks * slab_elems, src);
-        else if (lane == 0) tma_load_2d(sa, &tmA, &full_bar[stage], ks * slab_elems, w.m0);
         if (lane < bn / B_BOX_ROWS)
           tma_load_3d(sa + A_STAGE_BYTES + lane * B_BOX_BYTES, &tmB, &full_bar[stage], ks * slab_elems,
                       n0 + lane * B_BOX_ROWS, w.e);
@@ -255,6 +305,10 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       __syncwarp();
       if (++acc == NUM_ACC) { acc = 0; acc_phase ^= 1u; }
     }
+  } else if (kGather && warp >= ONE_THREADS / 32) {
+    // ------------------------------------------------------------------ gathering warps
+    gather_role<STAGES, STAGE_BYTES>(p, w, smem, empty_bar, abort_flag, warp - ONE_THREADS / 32, 0, int(blockIdx.x),
+                                     int(gridDim.x), num_tiles, [&](int s) { mbar_arrive(&full_bar[s]); });
   } else {
     // ------------------------------------------------------------------ epilogue
     const uint32_t lane_base = uint32_t(warp & 3) * 32u;
@@ -272,11 +326,9 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         if (kInt8) s_wscale[et] = inside ? __ldg(p.w_scale + (long long)w.e * p.N + n) : 0.f;
       }
       float a_scale = 1.f;
-      bool there = true;                                 // this row's index points into A (else: a row of zeros)
-      if (erow < w.rows) {
-        const int i = p.rows != nullptr ? __ldg(p.rows + w.m0 + erow) : w.m0 + erow;
-        there = i >= 0 && i < p.a_rows;
-        if (kInt8 && there) a_scale = __ldg(p.a_scale + i);
+      if (kInt8 && erow < w.rows) {
+        const int i = kGather ? __ldg(p.rows + w.m0 + erow) : w.m0 + erow;
+        if (i >= 0 && i < p.a_rows) a_scale = __ldg(p.a_scale + i);        // else: a row of zeros, whatever its scale
       }
       const bool got = mbar_wait(&acc_full[acc], acc_phase, abort_flag, p.status, 4);
       if (!epi_all(got)) break;                          // also publishes the column vectors
@@ -290,10 +342,6 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         uint32_t r[32];
         tmem_ld_32x32b_x32(t_addr + c * 64, r);
         tmem_ld_wait();
-        if (!there) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) r[j] = 0u;
-        }
         uint4 packed[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -333,22 +381,360 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 0 && *abort_flag) {                        // a wait gave up: see the copies in flight home first
-    for (uint32_t i = issued > STAGES ? issued - STAGES : 0u; i < issued; ++i)
-      for (uint32_t n = 0; n < 65536u && !mbar_try_wait(&full_bar[i % STAGES], (i / STAGES) & 1u); ++n) __nanosleep(64);
-  }
+  if (warp == 0 && *abort_flag) drain_copies<STAGES>(full_bar, issued);
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, TMEM_COLS);
   }
 }
 
+// ---------------------------------------------------------------------------------------------- CTA pairs
+// One MMA (M 256, N 256) issued by the pair's leader reads A and half of W from each CTA's shared memory.  Roles per
+// CTA: warp 0 W (and A) by TMA, warp 1 MMA issue (leader), kEpiWarps epilogue warps for the CTA's own 128 rows, an output
+// warp that sends each staged 64-column chunk and hands its staging tile back.  `full` lives in the leader, where both
+// CTAs' copies are counted.
+__host__ __device__ constexpr int pair_stages(bool int8) { return int8 ? 5 : 6; }
+__host__ __device__ constexpr int pair_out_bufs(bool int8) { return int8 ? 3 : 1; }
+constexpr int PAIR_STAGE_BYTES = A_STAGE_BYTES + (BN / 2) * SLAB_BYTES;
+__host__ __device__ constexpr int pair_epi_warps(bool int8) { return int8 ? 16 : 8; }
+__host__ __device__ constexpr int pair_smem_bytes(bool int8) {
+  return pair_stages(int8) * PAIR_STAGE_BYTES + pair_out_bufs(int8) * OUT_STAGE_BYTES + 2 * (kMaxExperts + 1) * 4 + 1024 + 256;
+}
+__host__ __device__ constexpr int pair_threads(bool int8) { return 96 + 32 * pair_epi_warps(int8); }
+
+template <int kType, bool kGelu>
+__global__ void __launch_bounds__(pair_threads(kType == kTypeI8), 1)
+grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                    const __grid_constant__ CUtensorMap tmOut, const GroupedParams p) {
+  constexpr bool kInt8 = kType == kTypeI8;
+  constexpr int STAGES = pair_stages(kInt8), OUT_BUFS = pair_out_bufs(kInt8), STAGE_BYTES = PAIR_STAGE_BYTES;
+  constexpr int kEpiWarps = pair_epi_warps(kInt8);
+  constexpr int CW = 64 / (kEpiWarps / 4);               // columns of a 64-column chunk per warp
+  constexpr int NV = CW / 8;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* stage_out0 = smem + STAGES * STAGE_BYTES;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(stage_out0 + OUT_BUFS * OUT_STAGE_BYTES);
+  uint64_t* empty_bar = full_bar + STAGES;
+  uint64_t* acc_full = empty_bar + STAGES;
+  uint64_t* acc_empty = acc_full + NUM_ACC;
+  uint64_t* stage_full = acc_empty + NUM_ACC;            // chunk staged by every epilogue warp, per staging tile
+  uint64_t* stage_free = stage_full + 3;                 // the chunk's store has read the staging tile
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(stage_free + 3);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* s_first = reinterpret_cast<int*>(tmem_slot + 2);
+  int* s_start = s_first + kMaxExperts + 1;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int pair = int(blockIdx.x >> 1), num_pairs = int(gridDim.x >> 1);
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < NUM_ACC; ++a) {
+      mbar_init(&acc_full[a], 1);
+      mbar_init(&acc_empty[a], 2 * kEpiWarps);
+    }
+    for (int b = 0; b < 3; ++b) {
+      mbar_init(&stage_full[b], kEpiWarps);
+      mbar_init(&stage_free[b], 1);
+    }
+    fence_mbar_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+    tma_prefetch_desc(&tmOut);
+  }
+  if (warp == 2) tile_list(p, 2 * BM, s_first, s_start);
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  constexpr int slab_elems = kInt8 ? SLAB_BYTES : SLAB_BYTES / 2;
+  const int tiles_n = (p.N + BN - 1) / BN;
+  const int num_tiles = s_first[p.E] * tiles_n;
+  const int skip = int(rank) * BM;                       // this CTA's first row of a tile
+  TileWalk w(s_first, s_start, tiles_n, 2 * BM);
+  uint32_t issued = 0;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      const uint32_t full0 = map_to_cta(&full_bar[0], 0);
+      uint32_t stage = 0, phase = 0;
+      bool ok = true;
+      for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
+        w.at(tile);
+        const int n0 = w.ntile * BN + int(rank) * (BN / 2);
+        for (int ks = 0; ks < p.k_slabs; ++ks) {
+          if (!(ok = mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, 1))) break;
+          uint8_t* sa = smem + stage * STAGE_BYTES;
+          if (rank == 0) mbar_expect_tx(&full_bar[stage], 2 * STAGE_BYTES);
+          tma_load_2d_pair(sa, &tmA, full0 + stage * 8, ks * slab_elems, w.m0 + skip);
+          tma_load_3d_pair(sa + A_STAGE_BYTES, &tmB, full0 + stage * 8, ks * slab_elems, n0, w.e);
+          ++issued;
+          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issue (leader)
+    if (rank == 0) {
+      const uint32_t fmt = kType == kTypeF16 ? kFmtF16 : kFmtBF16;
+      const uint32_t idesc = kInt8 ? make_idesc(kAccS32, kFmtS8, kFmtS8, 2 * BM, BN) : make_idesc(kAccF32, fmt, fmt, 2 * BM, BN);
+      const uint64_t desc0 = make_smem_desc(smem_u32(smem), 16, 1024, kSwizzle128B);
+      const uint32_t empty_own = map_to_cta(&empty_bar[0], 0), empty_peer = map_to_cta(&empty_bar[0], 1);
+      const uint32_t accf_own = map_to_cta(&acc_full[0], 0), accf_peer = map_to_cta(&acc_full[0], 1);
+      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+      bool ok = true;
+      for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[acc], acc_phase ^ 1u, abort_flag, p.status, 2)))) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + acc * BN;
+        for (int ks = 0; ks < p.k_slabs; ++ks) {
+          if (!(ok = __all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase, abort_flag, p.status, 3)))) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t adesc = desc0 + stage * (STAGE_BYTES / 16);
+            const uint64_t bdesc = adesc + A_STAGE_BYTES / 16;
+            const int nsteps = ks == p.k_slabs - 1 ? p.last_ksteps : 4;
+#pragma unroll
+            for (int k4 = 0; k4 < 4; ++k4) {
+              if (k4 >= nsteps) break;
+              const uint32_t accumulate = (ks | k4) != 0 ? 1u : 0u;
+              if (kInt8) umma_i8_ss_pair(d_tmem, adesc + k4 * 2, bdesc + k4 * 2, idesc, accumulate);
+              else umma_f16_ss_pair(d_tmem, adesc + k4 * 2, bdesc + k4 * 2, idesc, accumulate);
+            }
+            tc_commit_pair(empty_own + stage * 8);
+            tc_commit_pair(empty_peer + stage * 8);
+          }
+          __syncwarp();
+          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        }
+        if (!ok) break;
+        if (elect_one()) {
+          tc_commit_pair(accf_own + acc * 8);
+          tc_commit_pair(accf_peer + acc * 8);
+        }
+        __syncwarp();
+        if (++acc == NUM_ACC) { acc = 0; acc_phase ^= 1u; }
+      }
+    }
+  } else if (warp == 2 + kEpiWarps) {
+    // ------------------------------------------------------------------ output warp
+    // Staged chunk n of this CTA lives in staging tile n % OUT_BUFS.  Only whole halves are staged.
+    if (lane == 0) {
+      uint32_t n = 0;
+      bool ok = true;
+      for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
+        w.at(tile);
+        if (w.rows < skip + BM) continue;
+        const int n0 = w.ntile * BN;
+        for (int c = 0; c < BN / 64 && n0 + c * 64 < p.N; ++c, ++n) {
+          const uint32_t b = n % OUT_BUFS;
+          if (!(ok = mbar_wait(&stage_full[b], (n / OUT_BUFS) & 1u, abort_flag, p.status, 6))) break;
+          tma_store_2d(&tmOut, stage_out0 + b * OUT_STAGE_BYTES, n0 + c * 64, w.m0 + skip);
+          tma_store_commit();
+          // with several staging tiles, let this store run and hand back the tile of the one before it
+          tma_store_wait_read<(OUT_BUFS > 1 ? 1 : 0)>();
+          if (OUT_BUFS == 1) mbar_arrive(&stage_free[0]);
+          else if (n > 0) mbar_arrive(&stage_free[(n - 1) % OUT_BUFS]);
+        }
+      }
+      tma_store_wait_all<0>();
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue warps, own 128 rows
+    const uint32_t lane_base = uint32_t(warp & 3) * 32u;
+    const int qc = (warp - 2) >> 2;
+    const int erow = int(lane_base) + lane;
+    const uint32_t acc_empty0 = map_to_cta(&acc_empty[0], 0);
+    uint32_t acc = 0, acc_phase = 0, chunk_no = 0;
+    for (int tile = pair; tile < num_tiles; tile += num_pairs) {
+      w.at(tile);
+      const int n0 = w.ntile * BN;
+      const int mine = w.rows - skip;                    // rows of this CTA's half that exist (may be none)
+      const bool whole = mine >= BM;
+      const float* g_bias = p.bias != nullptr ? p.bias + (long long)w.e * p.N + n0 : nullptr;
+      const float* g_wscale = kInt8 ? p.w_scale + (long long)w.e * p.N + n0 : nullptr;
+      float a_scale = 1.f;
+      if (kInt8 && erow < mine) {
+        const int i = p.rows != nullptr ? __ldg(p.rows + w.m0 + skip + erow) : w.m0 + skip + erow;
+        if (i >= 0 && i < p.a_rows) a_scale = __ldg(p.a_scale + i);
+      }
+      if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[acc], acc_phase, abort_flag, p.status, 4))) break;
+      tc_fence_after();
+      const uint32_t t_addr = tmem_base + (lane_base << 16) + acc * BN + qc * CW;
+      // the tensor-memory load of chunk c + 1 is in flight while chunk c goes through the arithmetic, and the
+      // accumulator is handed back as soon as its last chunk is in registers
+      uint32_t rbuf[2][CW];
+      if constexpr (CW == 32) tmem_ld_32x32b_x32(t_addr, rbuf[0]);
+      else tmem_ld_32x32b_x16(t_addr, rbuf[0]);
+#pragma unroll
+      for (int c = 0; c < BN / 64; ++c) {
+        tmem_ld_wait();
+        if (c + 1 < BN / 64) {
+          if constexpr (CW == 32) tmem_ld_32x32b_x32(t_addr + (c + 1) * 64, rbuf[(c + 1) & 1]);
+          else tmem_ld_32x32b_x16(t_addr + (c + 1) * 64, rbuf[(c + 1) & 1]);
+        } else {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty0 + acc * 8);
+        }
+        if (n0 + c * 64 >= p.N || mine <= 0) continue;   // the same for the whole CTA
+        const uint32_t(&r)[CW] = rbuf[c & 1];
+        const uint32_t sbuf = chunk_no % OUT_BUFS, suse = chunk_no / OUT_BUFS;
+        uint8_t* stage_out = stage_out0 + sbuf * OUT_STAGE_BYTES;
+        bool ready = true;
+        if (whole && suse > 0) ready = mbar_test_wait(&stage_free[sbuf], (suse - 1u) & 1u);
+        uint4 packed[NV];
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+          const int ct0 = c * 64 + qc * CW + u * 8;
+          packed[u] = make_uint4(0u, 0u, 0u, 0u);
+          if (n0 + ct0 < p.N) {                          // N is a multiple of 8
+            float v[8];
+            if (g_bias != nullptr) epilogue8<kInt8, kInt8, true, kGelu>(r + u * 8, a_scale, g_wscale + ct0, g_bias + ct0, v);
+            else epilogue8<kInt8, kInt8, false, kGelu>(r + u * 8, a_scale, g_wscale + ct0, nullptr, v);
+            packed[u] = kType == kTypeF16 ? F16::pack(v) : Bf16::pack(v);
+          }
+        }
+        if (whole) {
+          if (!ready) mbar_wait(&stage_free[sbuf], (suse - 1u) & 1u, abort_flag, p.status, 7);
+          uint8_t* srow = stage_out + erow * 128;
+#pragma unroll
+          for (int u = 0; u < NV; ++u)
+            *reinterpret_cast<uint4*>(srow + (((qc * NV + u) ^ (erow & 7)) << 4)) = packed[u];
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&stage_full[sbuf]);
+          ++chunk_no;
+        } else if (erow < mine) {
+          // the last rows of an expert: straight from registers (one tile in many)
+          uint16_t* o = static_cast<uint16_t*>(p.out) + (w.m0 + skip + (long long)erow) * p.ldo + n0;
+#pragma unroll
+          for (int u = 0; u < NV; ++u) {
+            const int ct0 = c * 64 + qc * CW + u * 8;
+            if (n0 + ct0 < p.N) *reinterpret_cast<uint4*>(o + ct0) = packed[u];
+          }
+        }
+      }
+      if (++acc == NUM_ACC) { acc = 0; acc_phase ^= 1u; }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0 && lane == 0 && rank == 0 && *abort_flag) drain_copies<STAGES>(full_bar, issued);
+  cluster_sync_all();                                    // no CTA leaves while its peer may still signal it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, TMEM_COLS);
+  }
+}
+
+// Rows of A in the order of the slots, packed: 16-byte vectors, several loads a thread in flight.  A row that does not
+// exist is zeros; slots behind the last expert's are left out.
+constexpr int kOrderVecs = 4;
+__global__ void __launch_bounds__(256)
+order_rows_kernel(const GroupedParams p, uint4* __restrict__ to) {
+  const unsigned nv = unsigned(p.k_bytes >> 4);
+  const long long last = (long long)min(max(__ldg(p.offsets + p.E), 0), int(p.S)) * nv;
+  const long long i0 = (long long)blockIdx.x * (256 * kOrderVecs) + threadIdx.x;
+  uint4 v[kOrderVecs];
+#pragma unroll
+  for (int u = 0; u < kOrderVecs; ++u) {
+    const long long i = i0 + u * 256;
+    v[u] = make_uint4(0u, 0u, 0u, 0u);
+    if (i < last) {
+      const long long s = i / nv;
+      const int r = __ldg(p.rows + s);
+      if (r >= 0 && r < p.a_rows) v[u] = __ldg(reinterpret_cast<const uint4*>(p.a + r * p.a_pitch) + (i - s * nv));
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kOrderVecs; ++u)
+    if (i0 + u * 256 < last) to[i0 + u * 256] = v[u];
+}
+
 using GroupedFn = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const GroupedParams);
+
+template <int kType>
+GroupedFn one_of(bool gelu, bool gather) {
+  if (gelu) return gather ? grouped_one_kernel<kType, true, true> : grouped_one_kernel<kType, true, false>;
+  return gather ? grouped_one_kernel<kType, false, true> : grouped_one_kernel<kType, false, false>;
+}
+GroupedFn one_kernel(int type, bool gelu, bool gather) {
+  return type == kTypeBf16 ? one_of<kTypeBf16>(gelu, gather) : type == kTypeF16 ? one_of<kTypeF16>(gelu, gather) : one_of<kTypeI8>(gelu, gather);
+}
+GroupedFn pair_kernel(int type, bool gelu) {
+  if (type == kTypeBf16) return gelu ? grouped_pair_kernel<kTypeBf16, true> : grouped_pair_kernel<kTypeBf16, false>;
+  if (type == kTypeF16) return gelu ? grouped_pair_kernel<kTypeF16, true> : grouped_pair_kernel<kTypeF16, false>;
+  return gelu ? grouped_pair_kernel<kTypeI8, true> : grouped_pair_kernel<kTypeI8, false>;
+}
+
+// Rows per expert from which the pair kernel is the faster one.
+constexpr int64_t kPairRows = 192;
+
+bool want_pairs(int64_t S, int E) { return S >= kPairRows * int64_t(E); }
+
+int launch_pairs(int type, bool gelu, const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmOut,
+                 const GroupedParams& p, void* scratch, cudaStream_t st) {
+  const bool int8 = type == kTypeI8;
+  const GroupedFn kern = pair_kernel(type, gelu);
+  const int smem_bytes = pair_smem_bytes(int8);
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes) != cudaSuccess) return SAMB_E_LAUNCH;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.blockDim = dim3(unsigned(pair_threads(int8)));
+  cfg.dynamicSmemBytes = size_t(smem_bytes);
+  cfg.stream = st;
+  cfg.gridDim = dim3(unsigned(sm_count() & ~1));
+  static int cached_clusters[3][2] = {};                  // co-resident pairs per kernel variant (0 = not asked yet)
+  int& max_clusters = cached_clusters[type][gelu ? 1 : 0];
+  if (max_clusters == 0 &&
+      (cudaOccupancyMaxActiveClusters(&max_clusters, kern, &cfg) != cudaSuccess || max_clusters < 1)) {
+    cudaGetLastError();
+    max_clusters = -1;
+  }
+  if (max_clusters < 1) return SAMB_E_SHAPE;
+  if (p.rows != nullptr) {
+    const long long vecs = p.S * (p.k_bytes / 16);
+    const long long blocks = (vecs + 256 * kOrderVecs - 1) / (256 * kOrderVecs);
+    order_rows_kernel<<<unsigned(blocks), 256, 0, st>>>(p, static_cast<uint4*>(scratch));
+    if (int e = launch_status()) return e;
+  }
+  long long pairs = max_clusters < sm_count() / 2 ? max_clusters : sm_count() / 2;
+  const long long most = ((p.S + 2 * BM - 1) / (2 * BM) + p.E) * ((p.N + BN - 1) / BN);
+  if (most < pairs) pairs = most;
+  cfg.gridDim = dim3(unsigned(2 * pairs));
+  if (cudaLaunchKernelEx(&cfg, kern, tmA, tmB, tmOut, p) != cudaSuccess) {
+    cudaGetLastError();
+    return SAMB_E_LAUNCH;
+  }
+  return launch_status();
+}
 
 int launch_grouped(int type, const void* A, int64_t lda, int64_t a_rows, const float* a_scale, const int32_t* rows,
                    const void* W, int64_t ldw, int64_t w_stride, const float* w_scale, const float* bias,
                    const int32_t* offsets, void* out, int64_t ldo, int64_t S, int E, int N, int K, int epilogue,
-                   int32_t* status, void* stream) {
+                   void* scratch, int32_t* status, void* stream) {
   if (S < 0 || a_rows < 0 || E <= 0 || N <= 0 || K <= 0 || status == nullptr) return SAMB_E_BADARG;
   if (epilogue & ~(SAMB_EPI_BIAS | SAMB_EPI_GELU)) return SAMB_E_BADARG;
   if (((epilogue & SAMB_EPI_BIAS) != 0) != (bias != nullptr)) return SAMB_E_BADARG;
@@ -361,7 +747,8 @@ int launch_grouped(int type, const void* A, int64_t lda, int64_t a_rows, const f
   if (a_rows >= (int64_t(1) << 31) - BM || S >= (int64_t(1) << 31) - BM) return SAMB_E_SHAPE;
   // tile numbers are 32-bit, at the narrowest column tile
   if (((S + BM - 1) / BM + E) * ((N + 63) / 64) >= (int64_t(1) << 31)) return SAMB_E_SHAPE;
-  if ((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(W) | reinterpret_cast<uintptr_t>(out)) & 15u)
+  if ((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(W) | reinterpret_cast<uintptr_t>(out) |
+       reinterpret_cast<uintptr_t>(scratch)) & 15u)
     return SAMB_E_ALIGN;
   if ((reinterpret_cast<uintptr_t>(rows) | reinterpret_cast<uintptr_t>(offsets) | reinterpret_cast<uintptr_t>(bias) |
        reinterpret_cast<uintptr_t>(a_scale) | reinterpret_cast<uintptr_t>(w_scale)) & 3u)
@@ -373,18 +760,19 @@ int launch_grouped(int type, const void* A, int64_t lda, int64_t a_rows, const f
                                  : type == kTypeF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const uint32_t slab_elems = uint32_t(SLAB_BYTES / esz);
   CUtensorMap tmA, tmB, tmOut;
-  {
-    const uint64_t dims[2] = {uint64_t(K), uint64_t(a_rows)};
-    const uint64_t strides[2] = {uint64_t(esz), uint64_t(lda) * esz};
-    const uint32_t box[2] = {slab_elems, uint32_t(rows != nullptr ? 1 : BM)};
-    if (int e = make_tensor_map(&tmA, dt, 2, const_cast<void*>(A), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
-  }
-  {
+  auto map_a = [&](const void* base, int64_t ld, int64_t n) {
+    const uint64_t dims[2] = {uint64_t(K), uint64_t(n)};
+    const uint64_t strides[2] = {uint64_t(esz), uint64_t(ld) * esz};
+    const uint32_t box[2] = {slab_elems, uint32_t(BM)};
+    return make_tensor_map(&tmA, dt, 2, const_cast<void*>(base), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  // W in boxes of half a pair's column tile, or of the narrowest single-CTA one
+  auto map_w = [&](int box_rows) {
     const uint64_t dims[3] = {uint64_t(K), uint64_t(N), uint64_t(E)};
     const uint64_t strides[3] = {uint64_t(esz), uint64_t(ldw) * esz, uint64_t(E > 1 ? w_stride : ldw * N) * esz};
-    const uint32_t box[3] = {slab_elems, uint32_t(B_BOX_ROWS), 1};
-    if (int e = make_tensor_map(&tmB, dt, 3, const_cast<void*>(W), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
-  }
+    const uint32_t box[3] = {slab_elems, uint32_t(box_rows), 1};
+    return make_tensor_map(&tmB, dt, 3, const_cast<void*>(W), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  };
   {
     const uint64_t dims[2] = {uint64_t(N), uint64_t(S)};
     const uint64_t strides[2] = {2, uint64_t(ldo) * 2};
@@ -394,21 +782,30 @@ int launch_grouped(int type, const void* A, int64_t lda, int64_t a_rows, const f
       return e;
   }
   GroupedParams p;
-  p.out = out; p.bias = bias; p.a_scale = a_scale; p.w_scale = w_scale; p.rows = rows; p.offsets = offsets;
-  p.status = status;
-  p.ldo = ldo; p.a_rows = a_rows; p.S = S; p.E = E; p.N = N; p.K = K;
-  p.k_slabs = (K * esz + SLAB_BYTES - 1) / SLAB_BYTES;
-  p.last_ksteps = (K * esz - (p.k_slabs - 1) * SLAB_BYTES + 31) / 32;
-  p.gelu = (epilogue & SAMB_EPI_GELU) != 0;
-  static const GroupedFn kernels[3][2] = {{gemm_grouped_kernel<kTypeBf16, false>, gemm_grouped_kernel<kTypeBf16, true>},
-                                          {gemm_grouped_kernel<kTypeF16, false>, gemm_grouped_kernel<kTypeF16, true>},
-                                          {gemm_grouped_kernel<kTypeI8, false>, gemm_grouped_kernel<kTypeI8, true>}};
-  const GroupedFn kern = kernels[type][p.gelu];
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess)
+  p.out = out; p.a = static_cast<const uint8_t*>(A); p.bias = bias; p.a_scale = a_scale; p.w_scale = w_scale; p.rows = rows;
+  p.offsets = offsets; p.status = status;
+  p.ldo = ldo; p.a_rows = a_rows; p.S = S; p.a_pitch = lda * esz; p.E = E; p.N = N; p.K = K;
+  p.k_bytes = K * esz;
+  p.k_slabs = (p.k_bytes + SLAB_BYTES - 1) / SLAB_BYTES;
+  p.last_ksteps = (p.k_bytes - (p.k_slabs - 1) * SLAB_BYTES + 31) / 32;
+  const bool gelu = (epilogue & SAMB_EPI_GELU) != 0, gather = rows != nullptr;
+  auto st = static_cast<cudaStream_t>(stream);
+  // the pair kernel's epilogue reads the column vectors in 16-byte pieces; it wants its rows in order
+  if (want_pairs(S, E) && (!gather || scratch != nullptr) &&
+      !((reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(w_scale)) & 15u)) {
+    if (int e = gather ? map_a(scratch, K, S) : map_a(A, lda, a_rows)) return e;
+    if (int e = map_w(BN / 2)) return e;
+    const int e = launch_pairs(type, gelu, tmA, tmB, tmOut, p, scratch, st);
+    if (e != SAMB_E_SHAPE) return e;                     // pairs cannot be placed on this GPU: single CTAs
+  }
+  if (int e = map_a(A, lda, a_rows)) return e;
+  if (int e = map_w(B_BOX_ROWS)) return e;
+  const GroupedFn kern = one_kernel(type, gelu, gather);
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ONE_SMEM_BYTES) != cudaSuccess)
     return SAMB_E_LAUNCH;
   const long long most = ((S + BM - 1) / BM + E) * ((N + 63) / 64);
   const unsigned grid = unsigned(most < sm_count() ? most : sm_count());
-  kern<<<grid, NUM_THREADS, SMEM_BYTES, static_cast<cudaStream_t>(stream)>>>(tmA, tmB, tmOut, p);
+  kern<<<grid, ONE_THREADS + (gather ? 32 * ONE_STAGES : 0), ONE_SMEM_BYTES, st>>>(tmA, tmB, tmOut, p);
   return launch_status();
 }
 
@@ -417,19 +814,24 @@ int launch_grouped(int type, const void* A, int64_t lda, int64_t a_rows, const f
 
 extern "C" {
 
+int64_t samb_gemm_grouped_scratch_bytes(int64_t S, int E, int K, int is_i8) {
+  if (S <= 0 || E <= 0 || K <= 0 || !samb::want_pairs(S, E)) return 0;
+  return S * K * (is_i8 ? 1 : 2);
+}
+
 int samb_gemm_grouped(const void* A, int64_t lda, int64_t a_rows, const int32_t* rows, const void* W, int64_t ldw,
                       int64_t w_stride, const float* bias, const int32_t* offsets, void* out, int64_t ldo, int64_t S,
-                      int E, int N, int K, int is_f16, int epilogue, int32_t* status, void* stream) {
+                      int E, int N, int K, int is_f16, int epilogue, void* scratch, int32_t* status, void* stream) {
   return samb::launch_grouped(is_f16 ? samb::kTypeF16 : samb::kTypeBf16, A, lda, a_rows, nullptr, rows, W, ldw, w_stride,
-                              nullptr, bias, offsets, out, ldo, S, E, N, K, epilogue, status, stream);
+                              nullptr, bias, offsets, out, ldo, S, E, N, K, epilogue, scratch, status, stream);
 }
 
 int samb_gemm_i8_grouped(const int8_t* Aq, int64_t lda, int64_t a_rows, const float* a_scale, const int32_t* rows,
                          const int8_t* Wq, int64_t ldw, int64_t w_stride, const float* w_scale, const float* bias,
                          const int32_t* offsets, void* out, int64_t ldo, int64_t S, int E, int N, int K, int epilogue,
-                         int32_t* status, void* stream) {
+                         void* scratch, int32_t* status, void* stream) {
   return samb::launch_grouped(samb::kTypeI8, Aq, lda, a_rows, a_scale, rows, Wq, ldw, w_stride, w_scale, bias, offsets,
-                              out, ldo, S, E, N, K, epilogue, status, stream);
+                              out, ldo, S, E, N, K, epilogue, scratch, status, stream);
 }
 
 }  // extern "C"

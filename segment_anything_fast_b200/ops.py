@@ -750,7 +750,12 @@ def _grouped_args(a, w, offsets, rows, bias, out, out_dtype, kind):
         _need(out, out_dtype, "out")
         if out.shape != (S, N):
             raise RuntimeError(f"out: expected [{S}, {N}], got {list(out.shape)}")
-    return (lda, _indexes(rows, "rows", S) if rows is not None else None, w.stride(1) if N > 1 else K,
+    scratch = None
+    if rows is not None:                                  # room to put the rows of a large product in order
+        n = _lib.load().samb_gemm_grouped_scratch_bytes(S, E, K, a.dtype == torch.int8)
+        if n:
+            scratch = torch.empty(n, dtype=torch.uint8, device=a.device)
+    return (scratch, lda, _indexes(rows, "rows", S) if rows is not None else None, w.stride(1) if N > 1 else K,
             w.stride(0) if E > 1 else 0, _vector(bias, "bias", E, N), _indexes(offsets, "offsets", E + 1), out,
             _matrix(out, "out"), S, E, N, K)
 
@@ -763,11 +768,11 @@ def gemm_grouped(a: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows: 
     ``rows [S]`` as ``route_topk`` gives them.  Rows of ``out [S, N]`` behind the last expert's are left as they were
     (unspecified in a new ``out``); an index outside ``a`` stands for a row of zeros."""
     _need16(a, "a"); _need(w, a.dtype, "w")
-    lda, prow, ldw, ws, pbias, poff, out, ldo, S, E, N, K = _grouped_args(a, w, offsets, rows, bias, out, a.dtype,
-                                                                         "gemm_grouped")
+    scratch, lda, prow, ldw, ws, pbias, poff, out, ldo, S, E, N, K = _grouped_args(a, w, offsets, rows, bias, out,
+                                                                                  a.dtype, "gemm_grouped")
     _lib.check(_lib.load().samb_gemm_grouped(
         a.data_ptr(), lda, a.shape[0], prow, w.data_ptr(), ldw, ws, pbias, poff, out.data_ptr(), ldo, S, E, N, K,
-        a.dtype == torch.float16, (EPI_BIAS if bias is not None else 0) | (EPI_GELU if gelu else 0),
+        a.dtype == torch.float16, (EPI_BIAS if bias is not None else 0) | (EPI_GELU if gelu else 0), _ptr(scratch),
         status_word(a.device).data_ptr(), _stream()), "samb_gemm_grouped")
     return out
 
@@ -778,15 +783,15 @@ def gemm_i8_grouped(aq: torch.Tensor, a_scale: torch.Tensor, wq: torch.Tensor, w
     """``gemm_grouped`` on int8 ``aq [M, K]`` with row scales ``a_scale [M]`` (gathered with the rows) and ``wq [E, N, K]``
     with ``w_scale [E, N]``: exact int32 accumulation, bf16 out."""
     _need(aq, torch.int8, "aq"); _need(wq, torch.int8, "wq")
-    lda, prow, ldw, ws, pbias, poff, out, ldo, S, E, N, K = _grouped_args(aq, wq, offsets, rows, bias, out,
-                                                                         torch.bfloat16, "gemm_i8_grouped")
+    scratch, lda, prow, ldw, ws, pbias, poff, out, ldo, S, E, N, K = _grouped_args(aq, wq, offsets, rows, bias, out,
+                                                                                  torch.bfloat16, "gemm_i8_grouped")
     if a_scale is None or w_scale is None:
         raise RuntimeError("gemm_i8_grouped needs both scales")
     _lib.check(_lib.load().samb_gemm_i8_grouped(
         aq.data_ptr(), lda, aq.shape[0], _vector(a_scale, "a_scale", aq.shape[0]), prow, wq.data_ptr(), ldw, ws,
         _vector(w_scale, "w_scale", E, N), pbias, poff, out.data_ptr(), ldo, S, E, N, K,
-        (EPI_BIAS if bias is not None else 0) | (EPI_GELU if gelu else 0), status_word(aq.device).data_ptr(),
-        _stream()), "samb_gemm_i8_grouped")
+        (EPI_BIAS if bias is not None else 0) | (EPI_GELU if gelu else 0), _ptr(scratch),
+        status_word(aq.device).data_ptr(), _stream()), "samb_gemm_i8_grouped")
     return out
 
 

@@ -70,8 +70,8 @@ def test_route_refusals(lib, want, change):
 
 
 def _grouped(lib, a=P, lda=64, m=100, rows=P, w=P, ldw=64, ws=64 * 32, bias=P, off=P, out=P, ldo=32, S=200, E=4, N=32, K=64,
-             epi=1, st=P):
-    return lib.samb_gemm_grouped(a, lda, m, rows, w, ldw, ws, bias, off, out, ldo, S, E, N, K, 0, epi, st, None)
+             epi=1, st=P, scr=None):
+    return lib.samb_gemm_grouped(a, lda, m, rows, w, ldw, ws, bias, off, out, ldo, S, E, N, K, 0, epi, scr, st, None)
 
 
 @pytest.mark.parametrize("want,change", [
@@ -81,14 +81,14 @@ def _grouped(lib, a=P, lda=64, m=100, rows=P, w=P, ldw=64, ws=64 * 32, bias=P, o
     (SHAPE, dict(N=36, ldo=40)), (SHAPE, dict(K=60)), (SHAPE, dict(lda=56)), (SHAPE, dict(ldw=60)), (SHAPE, dict(ldo=24)),
     (SHAPE, dict(ws=64 * 16)), (SHAPE, dict(rows=None)), (SHAPE, dict(E=513)), (SHAPE, dict(S=(1 << 31) - 1)),
     (SHAPE, dict(S=(1 << 31) - 200, N=1 << 20, ldo=1 << 20, ws=1 << 26)),
-    (ALIGN, dict(a=P + 8)), (ALIGN, dict(out=P + 2)), (ALIGN, dict(off=P + 1)), (ALIGN, dict(rows=P + 2))])
+    (ALIGN, dict(a=P + 8)), (ALIGN, dict(scr=P + 8)), (ALIGN, dict(out=P + 2)), (ALIGN, dict(off=P + 1)), (ALIGN, dict(rows=P + 2))])
 def test_grouped_refusals(lib, want, change):
     assert _grouped(lib, **change) == want
 
 
 def test_grouped_i8_refusals(lib):
     def call(scale=P, ws=P, K=64):
-        return lib.samb_gemm_i8_grouped(P, 64, 100, scale, P, P, 64, 64 * 32, ws, None, P, P, 32, 200, 4, 32, K, 0, P, None)
+        return lib.samb_gemm_i8_grouped(P, 64, 100, scale, P, P, 64, 64 * 32, ws, None, P, P, 32, 200, 4, 32, K, 0, None, P, None)
     assert call(scale=None) == BAD and call(ws=None) == BAD
     assert call(K=56) == SHAPE                       # 8-element steps are enough for 16-bit types only
 
@@ -139,6 +139,12 @@ def test_rotary_freqs():
                 dict(rot=8, axes=3), dict(rot=8, base=0.0)):
         with pytest.raises(RuntimeError):
             ops.rotary_freqs(device=cpu, **bad)
+
+
+def test_grouped_scratch(lib):
+    f = lib.samb_gemm_grouped_scratch_bytes
+    assert f(2, 16, 1280, 0) == 0 and f(0, 1, 64, 0) == 0
+    assert f(65536, 16, 1280, 0) == 65536 * 1280 * 2 and f(1 << 30, 8, 5120, 1) == 5120 << 30
 
 
 def test_route_scratch(lib):

@@ -425,6 +425,34 @@ def test_gemm_grouped_bad_indexes(ops, S, t):
     ops.check_status()
 
 
+@pytest.mark.parametrize("t", [BF16, torch.int8])
+def test_gemm_grouped_without_scratch_and_with_an_odd_bias(ops, t):
+    """A product large enough for CTA pairs whose caller has no scratch, or whose bias starts at an odd place."""
+    from segment_anything_fast_b200 import _lib
+    g = gen(12)
+    S, M, E, N, K = 1500, 700, 3, 264, 160
+    a, w, sa, sw = operands(g, t, M, E, N, K)
+    rows = torch.randint(0, M, (S,), generator=g, device="cuda", dtype=torch.int32)
+    off = torch.tensor([0, 400, 1200, 1490], dtype=torch.int32, device="cuda")
+    bias = rand(g, E * N + 1)[1:].reshape(E, N)
+    want, slack, written = grouped64(a, w, off, rows, bias, True, S, sa, sw)
+    got = call_grouped(ops, a, w, sa, sw, off, rows=rows, bias=bias, gelu=True)
+    near(got[written], want[written], slack[written])
+    lib, st, out = _lib.load(), ops.status_word(a.device), torch.full((S, N), 7.0, dtype=BF16, device="cuda")
+    tail = (_lib.EPI_BIAS | _lib.EPI_GELU, None, st.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    bias = bias.clone()
+    if t == torch.int8:
+        rc = lib.samb_gemm_i8_grouped(a.data_ptr(), K, M, sa.data_ptr(), rows.data_ptr(), w.data_ptr(), K, N * K, sw.data_ptr(),
+                                      bias.data_ptr(), off.data_ptr(), out.data_ptr(), N, S, E, N, K, *tail)
+    else:
+        rc = lib.samb_gemm_grouped(a.data_ptr(), K, M, rows.data_ptr(), w.data_ptr(), K, N * K, bias.data_ptr(), off.data_ptr(),
+                                   out.data_ptr(), N, S, E, N, K, 0, *tail)
+    assert rc == 0
+    near(out[written], want[written], slack[written])
+    assert (out[~written] == 7.0).all()
+    ops.check_status()
+
+
 @pytest.mark.parametrize("S", [4, 300])
 def test_gemm_grouped_tells_rows_and_columns_apart(ops, S):
     """One-hot operands: every output says which row, column and expert it came from."""
