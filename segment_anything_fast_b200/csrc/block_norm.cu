@@ -4,12 +4,15 @@
 // of G equal blocks of rows (images).  y is computed from the fp32 x', not from its rounded copy: x' and y are each
 // rounded once.
 //
-// A thread owns eight fixed columns and walks down the rows, kRows of them at a time, so the affine parameters and
-// the gate (20 bytes a column against the 8 bytes a column that a row moves) stay in its registers.  A block is as
-// many warps as the width needs.  Statistics: a warp reduces its own 256 columns in two passes (mean, then squared
-// distances from it), and the warps' pairs (mean, M2) are joined by the parallel-variance formula
+// A thread owns eight fixed columns and walks down the rows, four at a time, so the affine parameters and the gate (20
+// bytes a column against the 8 bytes a column that a row moves) stay in its registers.  A block is as many warps as
+// the width needs; the next four rows are on their way into shared memory (16-byte cp.async, each thread reads back
+// what it copied) while four are worked on.
+// Statistics: a warp reduces its own 256 columns in two passes (mean, then squared distances from it), and the
+// warps' pairs (mean, M2) are joined by the parallel-variance formula
 //   M2 = sum_w M2_w + n_w (mean_w - mean)^2,
-// so a norm costs one block barrier for kRows rows and no difference of large squares is ever taken.
+// so a norm costs one block barrier for four rows and no difference of large squares is ever taken.  The four rows'
+// sums share their shuffles: halves of the warp trade rows first, 6 shuffles instead of 20.
 #include "elem16.cuh"
 
 namespace samb {
@@ -111,8 +114,217 @@ __device__ __forceinline__ void row_stats(const float (&v)[kRows][8], bool live,
   }
 }
 
-// kWide: up to 32 warps a block (C up to 8192), which leaves 64 registers a thread: the parameters are then read
-// where they are used.
+// The sum over the warp of four values: afterwards the lanes of group l >> 3 all hold the sum of value l >> 3.
+__device__ __forceinline__ float warp_sum4(const float (&v)[4]) {
+  const int lane = threadIdx.x & 31;
+  const bool upper = (lane & 16) != 0, odd = (lane & 8) != 0;
+  const float a = (upper ? v[2] : v[0]) + __shfl_xor_sync(0xffffffffu, upper ? v[0] : v[2], 16);
+  const float b = (upper ? v[3] : v[1]) + __shfl_xor_sync(0xffffffffu, upper ? v[1] : v[3], 16);
+  float c = (odd ? b : a) + __shfl_xor_sync(0xffffffffu, odd ? a : b, 8);
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+  return c;
+}
+
+// row_stats for four rows held as packed pairs and at most eight warps: lane l works on row l >> 3, and on warp l & 7
+// when the warps' results are joined.
+template <bool kRms>
+__device__ __forceinline__ void row_stats4(const f32x2 (&v)[4][4], bool live, int C, float eps, float2* stat,
+                                           float (&sub)[4], float (&mul)[4]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  float part[4], mean = 0.f;
+  if (!kRms) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float lo, hi;
+      unpack2(fadd2(fadd2(v[i][0], v[i][1]), fadd2(v[i][2], v[i][3])), lo, hi);
+      part[i] = live ? lo + hi : 0.f;
+    }
+    mean = warp_sum4(part) * (1.0f / float(min(256, C - warp * 256)));
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float m = kRms ? 0.f : __shfl_sync(0xffffffffu, mean, i * 8);
+    const f32x2 m2 = pack2(m, m);
+    f32x2 q = pack2(0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x2 d = kRms ? v[i][j] : fsub2(v[i][j], m2);
+      q = ffma2(d, d, q);
+    }
+    float lo, hi;
+    unpack2(q, lo, hi);
+    part[i] = live ? lo + hi : 0.f;
+  }
+  float m2 = warp_sum4(part);
+  if (warps > 1) {
+    if ((lane & 7) == 0) stat[warp * 4 + (lane >> 3)] = make_float2(mean, m2);
+    __syncthreads();
+    const int w = lane & 7;
+    const float2 s = w < warps ? stat[w * 4 + (lane >> 3)] : make_float2(0.f, 0.f);
+    const float n = w < warps ? float(min(256, C - w * 256)) : 0.f;
+    if (!kRms) {                                         // around the first warp's: a constant row stays exact
+      const float first = __shfl_sync(0xffffffffu, s.x, lane & 24);
+      float t = w < warps ? (s.x - first) * n : 0.f;
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+      mean = fmaf(t, 1.0f / float(C), first);
+    }
+    const float d = s.x - mean;
+    m2 = kRms ? s.y : fmaf(d * d, n, s.y);
+    if (w >= warps) m2 = 0.f;                            // also where the mean is not a number
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) m2 += __shfl_xor_sync(0xffffffffu, m2, o);
+  }
+  const float r = rsqrtf(fmaf(m2, 1.0f / float(C), eps));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    sub[i] = kRms ? 0.f : __shfl_sync(0xffffffffu, mean, i * 8);
+    mul[i] = __shfl_sync(0xffffffffu, r, i * 8);
+  }
+}
+
+__device__ __forceinline__ void cp_async_16(uint32_t smem_dst, const void* gsrc) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_dst), "l"(gsrc) : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack_pairs(const uint4& u, f32x2 (&v)[4]) {
+  float f[8];
+  T::unpack(u, f);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = pack2(f[2 * j], f[2 * j + 1]);
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack_pairs(const f32x2 (&v)[4]) {
+  float f[8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) unpack2(v[j], f[2 * j], f[2 * j + 1]);
+  return T::pack(f);
+}
+
+// Four rows at a time, at most eight warps (C up to 2048), the next four rows in flight.
+template <typename T, bool kRms, bool kQuant>
+__global__ void __launch_bounds__(256, 2)
+block_norm_rows_kernel(const NormParams p) {
+  extern __shared__ uint4 ring[];                        // [2 turns][h, r][4 rows][thread]
+  __shared__ float2 s_post[2][32], s_pre[2][32];
+  __shared__ float s_max[32];
+  const int threads = blockDim.x, c = int(threadIdx.x) * 8;
+  const bool live = c < p.C;
+  const int begin = int(blockIdx.x) * p.rows_per_block;
+  const int end = min(p.rows, begin + p.rows_per_block);
+  const bool has_post = p.post_g != nullptr, has_pre = p.pre_g != nullptr, has_res = p.r != nullptr;
+  uint4* mine = ring + threadIdx.x;
+  const uint16_t* h = static_cast<const uint16_t*>(p.h) + c;
+  const uint16_t* r = static_cast<const uint16_t*>(p.r) + c;
+  auto fetch = [&](int row0, int turn) {
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (row0 + i >= end) break;
+        cp_async_16(smem_u32(mine + ((turn * 2 + 0) * 4 + i) * threads), h + (row0 + i) * p.ldh);
+        if (has_res) cp_async_16(smem_u32(mine + ((turn * 2 + 1) * 4 + i) * threads), r + (row0 + i) * p.ldr);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  fetch(begin, 0);
+
+  f32x2 pg[4], pb[4], qg[4], qb[4];          // post's gain and offset (times the gate), pre's gain and offset
+  auto load4 = [&](const float* v, float other, f32x2 (&to)[4]) {
+    float f[8];
+    fill8(f, other);
+    if (live && v != nullptr) load8(v, c, f);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) to[j] = pack2(f[2 * j], f[2 * j + 1]);
+  };
+  load4(p.pre_g, 1.f, qg);
+  load4(p.pre_b, 0.f, qb);
+  const f32x2 scale2 = pack2(p.res_scale, p.res_scale);
+  int next_gate = begin, turn = 0;           // next_gate: first row that needs another gate vector than the one held
+
+  for (int row0 = begin; row0 < end; row0 += 4, turn ^= 1) {
+    fetch(row0 + 4, turn ^ 1);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    f32x2 v[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool there = live && row0 + i < end;
+      unpack_pairs<T>(there ? mine[((turn * 2 + 0) * 4 + i) * threads] : make_uint4(0u, 0u, 0u, 0u), v[i]);
+    }
+    float sub[4], mul[4];
+    if (has_post) {
+      row_stats4<kRms>(v, live, p.C, p.eps, s_post[turn], sub, mul);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[i][j] = fmul2(kRms ? v[i][j] : fsub2(v[i][j], pack2(sub[i], sub[i])), pack2(mul[i], mul[i]));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = row0 + i;
+      if (row < end && row >= next_gate) {               // the same for every thread
+        load4(p.post_g, 1.f, pg);
+        load4(p.post_b, 0.f, pb);
+        if (p.gate != nullptr) {
+          f32x2 g[4];
+          load4(p.gate + (long long)(row / p.rows_per_gate) * p.C, 1.f, g);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            pg[j] = fmul2(pg[j], g[j]);
+            pb[j] = fmul2(pb[j], g[j]);
+          }
+        }
+        next_gate = (row / p.rows_per_gate + 1) * p.rows_per_gate;   // <= rows: whole blocks of rows
+      }
+      const bool there = live && row < end;
+      f32x2 res[4];
+      unpack_pairs<T>(there && has_res ? mine[((turn * 2 + 1) * 4 + i) * threads] : make_uint4(0u, 0u, 0u, 0u), res);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i][j] = ffma2(v[i][j], pg[j], ffma2(scale2, res[j], pb[j]));
+      if (there) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.x) + row * p.ldx + c) = pack_pairs<T>(v[i]);
+    }
+    if (!has_pre) continue;
+    row_stats4<kRms>(v, live, p.C, p.eps, s_pre[turn], sub, mul);
+    uint4 out[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f32x2 f[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        f[j] = ffma2(fmul2(kRms ? v[i][j] : fsub2(v[i][j], pack2(sub[i], sub[i])), pack2(mul[i], mul[i])), qg[j], qb[j]);
+      out[i] = pack_pairs<T>(f);
+      if (!kQuant && live && row0 + i < end)
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.y) + (long long)(row0 + i) * p.C + c) = out[i];
+    }
+    if (kQuant) {
+      // the rounded row, as a quantised Linear fed with 16-bit rows would see it
+      const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = threads >> 5;
+      float amax[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        amax[i] = warp_max(live ? absmax_fold(absmax8(__floats2bfloat162_rn(0.f, 0.f), out[i])) : 0.f);
+        if (warps > 1 && lane == 0) s_max[warp * 4 + i] = amax[i];
+      }
+      if (warps > 1) __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        for (int w = 0; warps > 1 && w < warps; ++w) amax[i] = fmaxf(amax[i], s_max[w * 4 + i]);
+        float sc, inv_sc;
+        row_scale(amax[i], sc, inv_sc);
+        if (row0 + i < end) {
+          if (threadIdx.x == 0) p.y_scale[row0 + i] = sc;
+          if (live)
+            *reinterpret_cast<uint2*>(static_cast<int8_t*>(p.y) + (long long)(row0 + i) * p.C + c) = quant8(out[i], sc, inv_sc);
+        }
+      }
+    }
+  }
+}
+
+// One row at a time: few rows, where latency counts, and wide ones.  kWide: up to 32 warps a block (C up to 8192), which
+// leaves 64 registers a thread: the parameters are then read where they are used.
 template <typename T, bool kRms, bool kQuant, int kRows, bool kWide>
 __global__ void __launch_bounds__(kWide ? 1024 : 256)
 block_norm_kernel(const NormParams p) {
@@ -227,22 +439,35 @@ block_norm_kernel(const NormParams p) {
 
 template <typename T, bool kRms, bool kQuant>
 int launch_typed(NormParams& p, cudaStream_t st) {
-  const int warps = (p.C + 255) / 256;
+  const int warps = (p.C + 255) / 256, threads = warps * 32;
   const bool wide = warps > 8;
-  const int per_sm = wide ? 1 : 2048 / (warps * 32) < 4 ? 2048 / (warps * 32) : 4;
-  const long long slots = (long long)sm_count() * per_sm;
-  long long per_block = (p.rows + slots - 1) / slots;
-  if (!wide && per_block >= 4) {
-    per_block = (per_block + 3) / 4 * 4;
-    p.rows_per_block = int(per_block);
-    const unsigned blocks = unsigned((p.rows + per_block - 1) / per_block);
-    block_norm_kernel<T, kRms, kQuant, 4, false><<<blocks, warps * 32, 0, st>>>(p);
-  } else {
-    p.rows_per_block = int(per_block);
-    const unsigned blocks = unsigned((p.rows + per_block - 1) / per_block);
-    if (wide) block_norm_kernel<T, kRms, kQuant, 1, true><<<blocks, warps * 32, 0, st>>>(p);
-    else block_norm_kernel<T, kRms, kQuant, 1, false><<<blocks, warps * 32, 0, st>>>(p);
+  const int smem = 2 * 2 * 4 * threads * int(sizeof(uint4));
+  auto rows4 = block_norm_rows_kernel<T, kRms, kQuant>;
+  static int cached_blocks[9] = {0};                     // resident blocks per SM by warps (a device fact, asked once)
+  int blocks_sm = 0;
+  if (!wide) {
+    if (smem > 48 * 1024 && cudaFuncSetAttribute(rows4, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+      return SAMB_E_LAUNCH;
+    int& n = cached_blocks[warps];
+    if (n == 0) {
+      int got = 0;
+      if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&got, rows4, threads, size_t(smem)) != cudaSuccess || got < 1)
+        return SAMB_E_LAUNCH;
+      n = got;
+    }
+    blocks_sm = n;
   }
+  const long long slots = (long long)sm_count() * blocks_sm;
+  if (!wide && p.rows >= 4 * slots) {                    // four rows for every resident block: one resident wave
+    p.rows_per_block = int(((p.rows + slots - 1) / slots + 3) / 4 * 4);
+    rows4<<<unsigned((p.rows + p.rows_per_block - 1) / p.rows_per_block), threads, smem, st>>>(p);
+    return launch_status();
+  }
+  const long long most = (long long)sm_count() * (wide ? 2 : 8);
+  p.rows_per_block = int((p.rows + most - 1) / most);
+  const unsigned blocks = unsigned((p.rows + p.rows_per_block - 1) / p.rows_per_block);
+  if (wide) block_norm_kernel<T, kRms, kQuant, 1, true><<<blocks, threads, 0, st>>>(p);
+  else block_norm_kernel<T, kRms, kQuant, 1, false><<<blocks, threads, 0, st>>>(p);
   return launch_status();
 }
 
