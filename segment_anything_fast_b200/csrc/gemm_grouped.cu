@@ -3,9 +3,10 @@
 // The offsets live on the device (the router wrote them), so the host launches one wave of persistent CTAs and every
 // CTA works the tile list out for itself: the prefix over the experts of their row tiles, times the column tiles.
 //
-// Two kernels.  On CTA pairs (256 x 256 tiles, cta_group::2, each CTA loads its 128 rows of A and half of W) for groups
+// Three kernels.  On CTA pairs (256 x 256 tiles, cta_group::2, each CTA loads its 128 rows of A and half of W) for groups
 // of a few hundred rows and more; on single CTAs (128 x 256, 128 or 64) below, where the weights' bytes count and the
-// number of tiles is what spreads their stream over the SMs.
+// number of tiles is what spreads their stream over the SMs; and for a handful of rows in all (serving a token or two) dot
+// products by warps, which have neither tensor maps to build nor a pipeline to fill.
 //
 // Operands: 128-byte K slabs in a ring of 128B-swizzled stages, W by TMA, and A too when its rows lie in order.  With
 // `rows` the single-CTA kernel has a warp per stage fetch them with 16-byte cp.async into the same swizzled places.  The
@@ -643,6 +644,174 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   }
 }
 
+// ---------------------------------------------------------------------------------------------- a handful of rows
+// A warp owns RN neighbouring rows of one expert's W and multiplies them with up to four rows of A at a time: lanes split
+// K in 16-byte pieces, partial sums meet in shuffles.  Bound by the stream of weights (26 MB for one token with two
+// experts of 5120 x 1280): eight 16-byte loads a lane in flight, RN = 4, 2 or 1 so that some sixteen warps an SM share it.
+constexpr int FEW_WARPS = 8;
+
+template <int kType>
+struct Dot {                       // 16 bytes of both operands
+  using Acc = f32x2;
+  static __device__ __forceinline__ Acc zero() { return pack2(0.f, 0.f); }
+  static __device__ __forceinline__ Acc add(const uint4& a, const uint4& b, Acc c) {
+    const uint32_t u[4] = {a.x, a.y, a.z, a.w}, v[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (kType == kTypeF16) {
+        const float2 s = F16::unpack2f(u[j]), t = F16::unpack2f(v[j]);
+        c = ffma2(pack2(s.x, s.y), pack2(t.x, t.y), c);
+      } else {
+        c = ffma2(bf16x2_to_f32x2(u[j]), bf16x2_to_f32x2(v[j]), c);
+      }
+    }
+    return c;
+  }
+  static __device__ __forceinline__ float sum(Acc c) {
+    float lo, hi;
+    unpack2(c, lo, hi);
+    return lo + hi;
+  }
+};
+template <>
+struct Dot<kTypeI8> {
+  using Acc = int;
+  static __device__ __forceinline__ int zero() { return 0; }
+  static __device__ __forceinline__ int add(const uint4& a, const uint4& b, int c) {
+    c = __dp4a(int(a.x), int(b.x), c);
+    c = __dp4a(int(a.y), int(b.y), c);
+    c = __dp4a(int(a.z), int(b.z), c);
+    return __dp4a(int(a.w), int(b.w), c);
+  }
+  static __device__ __forceinline__ int sum(int c) { return c; }
+};
+
+// The nth expert that has rows (by one warp): its number or -1, its first slot and its rows, by the rules of tile_list.
+__device__ __forceinline__ int nth_expert(const GroupedParams& p, int nth, int& first, int& rows) {
+  const int lane = threadIdx.x & 31;
+  int at = 0;
+  for (int e0 = 0; e0 < p.E; e0 += 32) {
+    const int e = e0 + lane;
+    int lo = 0, hi = 0;
+    if (e < p.E) {
+      lo = min(max(__ldg(p.offsets + e), 0), int(p.S));
+      hi = min(max(__ldg(p.offsets + e + 1), 0), int(p.S));
+    }
+    int top = max(lo, hi);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, top, o);
+      if (lane >= o) top = max(top, up);
+    }
+    top = max(top, at);
+    int below = __shfl_up_sync(0xffffffffu, top, 1);
+    if (lane == 0) below = e0 == 0 ? lo : at;
+    const int begin = max(lo, below), n = max(0, hi - begin);
+    const unsigned have = __ballot_sync(0xffffffffu, n > 0);
+    if (__popc(have) > nth) {
+      const int src = __ffs(__ballot_sync(0xffffffffu, n > 0 && __popc(have & ((1u << lane) - 1u)) == nth)) - 1;
+      first = __shfl_sync(0xffffffffu, begin, src);
+      rows = __shfl_sync(0xffffffffu, n, src);
+      return e0 + src;
+    }
+    nth -= __popc(have);
+    at = __shfl_sync(0xffffffffu, top, 31);
+  }
+  return -1;
+}
+
+template <int kType, int RN>
+__global__ void __launch_bounds__(32 * FEW_WARPS)
+grouped_few_kernel(const uint8_t* __restrict__ W, const long long w_pitch, const long long w_stride, const GroupedParams p,
+                   const int gelu) {
+  constexpr bool kInt8 = kType == kTypeI8;
+  constexpr int TK = 4, UK = 8 / RN;                     // rows of A at a time; 16-byte steps of K in flight
+  using D = Dot<kType>;
+  const int lane = threadIdx.x & 31;
+  const int n0 = (int(blockIdx.x) * FEW_WARPS + int(threadIdx.x >> 5)) * RN;
+  if (n0 >= p.N) return;                                 // N is a multiple of 8: all RN rows exist
+  int first = 0, rows = 0;
+  const int e = nth_expert(p, int(blockIdx.y), first, rows);
+  if (e < 0) return;
+  const int steps = p.k_bytes >> 4;                      // 16-byte pieces of K
+  const uint8_t* w = W + e * w_stride + n0 * w_pitch;
+  for (int t0 = 0; t0 < rows; t0 += TK) {
+    const uint8_t* a[TK];
+    float scale[TK];
+#pragma unroll
+    for (int t = 0; t < TK; ++t) {
+      int i = -1;
+      if (t0 + t < rows) i = p.rows != nullptr ? __ldg(p.rows + first + t0 + t) : first + t0 + t;
+      const bool there = i >= 0 && i < p.a_rows;
+      a[t] = there ? p.a + i * p.a_pitch : nullptr;
+      scale[t] = kInt8 && there ? __ldg(p.a_scale + i) : 1.f;
+    }
+    typename D::Acc acc[TK][RN];
+#pragma unroll
+    for (int t = 0; t < TK; ++t)
+#pragma unroll
+      for (int r = 0; r < RN; ++r) acc[t][r] = D::zero();
+    for (int k0 = lane; k0 < steps; k0 += 32 * UK) {
+      uint4 wv[UK][RN];
+#pragma unroll
+      for (int u = 0; u < UK; ++u)
+#pragma unroll
+        for (int r = 0; r < RN; ++r)
+          wv[u][r] = k0 + u * 32 < steps ? __ldg(reinterpret_cast<const uint4*>(w + r * w_pitch) + k0 + u * 32)
+                                         : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int t = 0; t < TK; ++t) {
+        if (a[t] == nullptr) continue;                   // the same for the whole warp
+#pragma unroll
+        for (int u = 0; u < UK; ++u) {
+          if (k0 + u * 32 >= steps) break;
+          const uint4 av = __ldg(reinterpret_cast<const uint4*>(a[t]) + k0 + u * 32);
+#pragma unroll
+          for (int r = 0; r < RN; ++r) acc[t][r] = D::add(av, wv[u][r], acc[t][r]);
+        }
+      }
+    }
+    // lane t * RN + r finishes output (t, r)
+    float mine = 0.f;
+    float mine_scale = 1.f;
+#pragma unroll
+    for (int t = 0; t < TK; ++t)
+#pragma unroll
+      for (int r = 0; r < RN; ++r) {
+        auto v = D::sum(acc[t][r]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (lane == t * RN + r) {
+          mine = float(v);
+          mine_scale = scale[t];
+        }
+      }
+    const int t = lane / RN, n = n0 + lane % RN;
+    if (t < TK && t0 + t < rows) {
+      if (kInt8) mine = mine * mine_scale * __ldg(p.w_scale + (long long)e * p.N + n);
+      if (p.bias != nullptr) mine += __ldg(p.bias + (long long)e * p.N + n);
+      if (gelu) mine = gelu_erf(mine);
+      static_cast<uint16_t*>(p.out)[(first + t0 + t) * p.ldo + n] = kType == kTypeF16 ? F16::from_float(mine) : Bf16::from_float(mine);
+    }
+  }
+}
+
+template <int kType>
+void launch_few(const uint8_t* W, long long w_pitch, long long w_stride, const GroupedParams& p, bool gelu, cudaStream_t st) {
+  const unsigned groups = unsigned(p.S < p.E ? p.S : p.E);
+  const long long warps = (long long)p.N * groups, full = (long long)sm_count() * 16;
+  const int rn = warps >= 4 * full ? 4 : warps >= 2 * full ? 2 : 1;
+  const dim3 grid(unsigned((p.N + FEW_WARPS * rn - 1) / (FEW_WARPS * rn)), groups);
+  if (rn == 4) grouped_few_kernel<kType, 4><<<grid, 32 * FEW_WARPS, 0, st>>>(W, w_pitch, w_stride, p, gelu);
+  else if (rn == 2) grouped_few_kernel<kType, 2><<<grid, 32 * FEW_WARPS, 0, st>>>(W, w_pitch, w_stride, p, gelu);
+  else grouped_few_kernel<kType, 1><<<grid, 32 * FEW_WARPS, 0, st>>>(W, w_pitch, w_stride, p, gelu);
+}
+
+#ifndef SAMB_FEW_SLOTS
+#define SAMB_FEW_SLOTS 8
+#endif
+constexpr int64_t kFewSlots = SAMB_FEW_SLOTS;
+
 // Rows of A in the order of the slots, packed: 16-byte vectors, several loads a thread in flight.  A row that does not
 // exist is zeros; slots behind the last expert's are left out.
 constexpr int kOrderVecs = 4;
@@ -790,6 +959,14 @@ int launch_grouped(int type, const void* A, int64_t lda, int64_t a_rows, const f
   p.last_ksteps = (p.k_bytes - (p.k_slabs - 1) * SLAB_BYTES + 31) / 32;
   const bool gelu = (epilogue & SAMB_EPI_GELU) != 0, gather = rows != nullptr;
   auto st = static_cast<cudaStream_t>(stream);
+  if (S <= kFewSlots) {
+    const uint8_t* w = static_cast<const uint8_t*>(W);
+    const long long pitch = ldw * esz, stride = w_stride * esz;
+    if (type == kTypeBf16) launch_few<kTypeBf16>(w, pitch, stride, p, gelu, st);
+    else if (type == kTypeF16) launch_few<kTypeF16>(w, pitch, stride, p, gelu, st);
+    else launch_few<kTypeI8>(w, pitch, stride, p, gelu, st);
+    return launch_status();
+  }
   // the pair kernel's epilogue reads the column vectors in 16-byte pieces; it wants its rows in order
   if (want_pairs(S, E) && (!gather || scratch != nullptr) &&
       !((reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(w_scale)) & 15u)) {

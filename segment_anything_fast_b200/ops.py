@@ -14,7 +14,7 @@ _status_words = {}
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _same_device(index: Optional[int], name: str) -> None:
@@ -57,7 +57,7 @@ def _need(t: torch.Tensor, dtype: torch.dtype, name: str) -> None:
         raise RuntimeError(f"{name}: expected a CUDA tensor (there is no CPU path)")
     if t.dtype != dtype:
         raise RuntimeError(f"{name}: expected {dtype}, got {t.dtype}")
-    _same_device(t.device.index, name)
+    _same_device(t.get_device(), name)
 
 
 def _rows2d(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -542,66 +542,104 @@ def normalize_u8(x: torch.Tensor, mean, std, out: Optional[torch.Tensor] = None)
 # Operators of transformer blocks beside the reference's own kind: norms around a block, rotary positions, a mixture
 # of experts.  16-bit tensors are bfloat16 or float16.
 # ---------------------------------------------------------------------------------------------------------------
-_HALF = (torch.bfloat16, torch.float16)
+_F32, _F16, _BF16, _I32 = torch.float32, torch.float16, torch.bfloat16, torch.int32
 
 
-def _need16(t: torch.Tensor, name: str) -> None:
-    if t.dtype not in _HALF:
-        raise RuntimeError(f"{name}: expected bfloat16 or float16, got {t.dtype}")
-    _need(t, t.dtype, name)
+def _here(t: torch.Tensor, dtype: torch.dtype, dev: int, name: str) -> None:
+    """``_need`` against a device number that the caller has asked for once."""
+    if t.dtype is not dtype or t.get_device() != dev:
+        _need(t, dtype, name)
 
 
-def _vector(t: Optional[torch.Tensor], name: str, *shape: int) -> Optional[int]:
-    """Pointer of a contiguous fp32 tensor of this shape (or None)."""
-    if t is None:
-        return None
-    _need(t, torch.float32, name)
-    if tuple(t.shape) != shape or not t.is_contiguous():
+def _half(t: torch.Tensor, name: str) -> Tuple[torch.dtype, int]:
+    """Type and device of a bfloat16 or float16 tensor on the current device."""
+    dtype = t.dtype
+    if dtype is not _BF16 and dtype is not _F16:
+        raise RuntimeError(f"{name}: expected bfloat16 or float16, got {dtype}")
+    if not t.is_cuda:
+        _need(t, dtype, name)
+    dev = torch.cuda.current_device()
+    _here(t, dtype, dev, name)
+    return dtype, dev
+
+
+def _vector(t: torch.Tensor, name: str, dev: int, shape: Tuple[int, ...]) -> int:
+    """Pointer of a contiguous fp32 tensor of this shape."""
+    _here(t, _F32, dev, name)
+    if t.shape != shape or not t.is_contiguous():
         raise RuntimeError(f"{name}: expected a contiguous float32 tensor of shape {list(shape)}, got {list(t.shape)}")
     return t.data_ptr()
 
 
-def _indexes(t: torch.Tensor, name: str, n: int) -> int:
-    _need(t, torch.int32, name)
-    if t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+def _indexes(t: torch.Tensor, name: str, dev: int, n: int) -> int:
+    _here(t, _I32, dev, name)
+    if t.shape != (n,) or not t.is_contiguous():
         raise RuntimeError(f"{name}: expected a contiguous int32 tensor of {n} elements, got {list(t.shape)}")
     return t.data_ptr()
 
 
 def _matrix(t: torch.Tensor, name: str) -> int:
     """Leading dimension of a row-major matrix; a single row has none of its own."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise RuntimeError(f"{name}: expected a 2-D tensor with unit inner stride")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if t.dim() == 2:
+        rows, cols = t.shape
+        ld, inner = t.stride()
+        if inner == 1 or cols <= 1:
+            return ld if rows > 1 else cols
+    raise RuntimeError(f"{name}: expected a 2-D tensor with unit inner stride")
 
 
-def _block_norm_args(h, residual, post, pre, gate, out):
-    _need16(h, "h")
+def _like(t: torch.Tensor, dtype: torch.dtype, dev: int, shape, name: str) -> int:
+    """Leading dimension of a matrix that has to have this type and shape."""
+    _here(t, dtype, dev, name)
+    if t.shape != shape:
+        raise RuntimeError(f"{name}: expected shape {list(shape)}, got {list(t.shape)}")
+    return _matrix(t, name)
+
+
+def _block_norm(fn: str, h, residual, post, pre, gate, res_scale, eps, rms, out, quant):
+    dtype, dev = _half(h, "h")
     ldh = _matrix(h, "h")
-    rows, C = h.shape
-    ldr = 0
+    shape = h.shape
+    rows, C = shape
+    pr = pgg = pgb = pqg = pqb = pg = py = ps = None
+    ldr = gates = 0
     if residual is not None:
-        _need(residual, h.dtype, "residual")
-        ldr = _matrix(residual, "residual")
-        if residual.shape != h.shape:
-            raise RuntimeError("residual must have the shape of h")
-    if out is None:
-        out = torch.empty(rows, C, dtype=h.dtype, device=h.device)
-    else:
-        _need(out, h.dtype, "out")
-        if out.shape != h.shape:
-            raise RuntimeError("out must have the shape of h")
-    post_g, post_b = post if post is not None else (None, None)
-    pre_g, pre_b = pre if pre is not None else (None, None)
-    gate_rows = 0
+        ldr = _like(residual, dtype, dev, shape, "residual")
+        pr = residual.data_ptr()
+    if post is not None:
+        gain, offset = post
+        pgg = _vector(gain, "post gain", dev, (C,))
+        if offset is not None:
+            pgb = _vector(offset, "post offset", dev, (C,))
+    if pre is not None:
+        gain, offset = pre
+        pqg = _vector(gain, "pre gain", dev, (C,))
+        if offset is not None:
+            pqb = _vector(offset, "pre offset", dev, (C,))
     if gate is not None:
-        gate_rows = gate.shape[0] if gate.dim() == 2 else 1
-        if gate_rows == 0 or rows % gate_rows:
-            raise RuntimeError(f"gate: {gate_rows} vectors do not divide {rows} rows")
-    args = (h.data_ptr(), ldh, _ptr(residual), ldr, _vector(post_g, "post gain", C), _vector(post_b, "post offset", C),
-            _vector(pre_g, "pre gain", C), _vector(pre_b, "pre offset", C),
-            _vector(gate, "gate", *((gate_rows, C) if gate is not None and gate.dim() == 2 else (C,))), gate_rows)
-    return args, out, _matrix(out, "out"), rows, C
+        gates = gate.shape[0] if gate.dim() == 2 else 1
+        pg = _vector(gate, "gate", dev, (gates, C) if gate.dim() == 2 else (C,))
+        if gates == 0 or rows % gates:
+            raise RuntimeError(f"gate: {gates} vectors do not divide {rows} rows")
+    if out is None:
+        out, ldx = torch.empty((rows, C), dtype=dtype, device=h.device), C
+    else:
+        ldx = _like(out, dtype, dev, shape, "out")
+    y = scale = None
+    if quant:
+        y = torch.empty((rows, C), dtype=torch.int8, device=h.device)
+        scale = torch.empty((rows,), dtype=_F32, device=h.device)
+        _lib.check(_lib.load().samb_block_norm_quant_i8(
+            h.data_ptr(), ldh, pr, ldr, pgg, pgb, pqg, pqb, pg, gates, res_scale, eps, rms, out.data_ptr(), ldx,
+            y.data_ptr(), scale.data_ptr(), rows, C, _stream()), fn)
+    else:
+        if pre is not None:
+            y = torch.empty((rows, C), dtype=dtype, device=h.device)
+            py = y.data_ptr()
+        _lib.check(_lib.load().samb_block_norm(
+            h.data_ptr(), ldh, pr, ldr, pgg, pgb, pqg, pqb, pg, gates, res_scale, eps, dtype is _F16, rms,
+            out.data_ptr(), ldx, py, rows, C, _stream()), fn)
+    return out, y, scale
 
 
 def block_norm(h: torch.Tensor, residual: Optional[torch.Tensor] = None, post=None, pre=None,
@@ -612,11 +650,7 @@ def block_norm(h: torch.Tensor, residual: Optional[torch.Tensor] = None, post=No
     ``pre``.  ``post`` / ``pre`` are ``(gain, offset or None)`` in fp32, LayerNorm or with ``rms`` root-mean-square
     norms; ``gate`` is fp32 ``[C]``, or ``[G, C]`` with one vector for each of G equal blocks of rows.  ``out`` (x) may
     be ``residual`` or ``h``."""
-    args, out, ldx, rows, C = _block_norm_args(h, residual, post, pre, gate, out)
-    y = torch.empty(rows, C, dtype=h.dtype, device=h.device) if pre is not None else None
-    _lib.check(_lib.load().samb_block_norm(*args, res_scale, eps, h.dtype == torch.float16, rms, out.data_ptr(), ldx,
-                                           _ptr(y), rows, C, _stream()), "samb_block_norm")
-    return out, y
+    return _block_norm("samb_block_norm", h, residual, post, pre, gate, res_scale, eps, rms, out, False)[:2]
 
 
 def block_norm_quant_i8(h: torch.Tensor, residual: Optional[torch.Tensor], post, pre, gate: Optional[torch.Tensor] = None,
@@ -627,12 +661,7 @@ def block_norm_quant_i8(h: torch.Tensor, residual: Optional[torch.Tensor], post,
     _need(h, torch.bfloat16, "h")
     if pre is None:
         raise RuntimeError("block_norm_quant_i8 needs the norm whose output it quantises")
-    args, out, ldx, rows, C = _block_norm_args(h, residual, post, pre, gate, out)
-    yq = torch.empty(rows, C, dtype=torch.int8, device=h.device)
-    scale = torch.empty(rows, dtype=torch.float32, device=h.device)
-    _lib.check(_lib.load().samb_block_norm_quant_i8(*args, res_scale, eps, rms, out.data_ptr(), ldx, yq.data_ptr(),
-                                                    scale.data_ptr(), rows, C, _stream()), "samb_block_norm_quant_i8")
-    return out, yq, scale
+    return _block_norm("samb_block_norm_quant_i8", h, residual, post, pre, gate, res_scale, eps, rms, out, True)
 
 
 def rotary_freqs(rot: int, base: float = 10000.0, axes: int = 1, scaling: Optional[str] = None, factor: float = 1.0,
@@ -671,32 +700,41 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, interl
     neighbours (``interleaved``) or half the rotated width apart; the first ``2 * len(freqs)`` elements of a row turn,
     the rest is copied.  ``positions`` int32 / int64: ``[P]``, or ``[P, 2]`` for a raster (first half of the pairs by the
     first coordinate); row r uses entry ``r % P``.  ``freqs`` float64, see ``rotary_freqs``.  ``out`` may be ``x``."""
-    _need16(x, "x")
-    _need(freqs, torch.float64, "freqs")
-    if positions.dtype not in (torch.int32, torch.int64):
-        raise RuntimeError(f"positions: expected int32 or int64, got {positions.dtype}")
-    _need(positions, positions.dtype, "positions")
-    if x.dim() != 3 or (x.shape[2] > 1 and x.stride(2) != 1):
-        raise RuntimeError("x: expected a [planes, rows, d] tensor with unit inner stride")
+    dtype, dev = _half(x, "x")
+    _here(freqs, torch.float64, dev, "freqs")
+    pt = positions.dtype
+    if pt is not torch.int64 and pt is not _I32:
+        raise RuntimeError(f"positions: expected int32 or int64, got {pt}")
+    _here(positions, pt, dev, "positions")
+    if x.dim() != 3:
+        raise RuntimeError("x: expected a [planes, rows, d] tensor")
     planes, rows, d = x.shape
-    if positions.dim() not in (1, 2) or not positions.is_contiguous() or (positions.dim() == 2 and positions.shape[1] != 2):
+    ps, rs, es = x.stride()
+    axes = positions.dim()
+    if axes not in (1, 2) or not positions.is_contiguous() or (axes == 2 and positions.shape[1] != 2):
         raise RuntimeError("positions: expected a contiguous [P] or [P, 2] tensor")
-    period, axes = positions.shape[0], positions.dim()
+    period = positions.shape[0]
     if rows and (period == 0 or rows % period):
         raise RuntimeError(f"positions: {period} entries do not divide {rows} rows")
     if freqs.dim() != 1 or not freqs.is_contiguous():
         raise RuntimeError("freqs: expected a contiguous 1-D tensor")
     if out is None:
-        out = torch.empty(planes, rows, d, dtype=x.dtype, device=x.device)
-    elif out is not x:
-        _need(out, x.dtype, "out")
-        if out.shape != x.shape or (d > 1 and out.stride(2) != 1):
-            raise RuntimeError("out must have the shape of x and unit inner stride")
+        out = torch.empty((planes, rows, d), dtype=dtype, device=x.device)
+        ops_, ors, oes = rows * d, d, 1
+    else:
+        _here(out, dtype, dev, "out")
+        if out.shape != x.shape:
+            raise RuntimeError("out must have the shape of x")
+        ops_, ors, oes = out.stride()
+    if d > 1 and (es != 1 or oes != 1):
+        raise RuntimeError("x and out: expected unit inner stride")
+    if planes <= 1:                                       # strides of a single plane or row mean nothing
+        ps = ops_ = 0
+    if rows <= 1:
+        rs = ors = 0
     _lib.check(_lib.load().samb_rotary(
-        x.data_ptr(), x.stride(0) if planes > 1 else 0, x.stride(1) if rows > 1 else 0, positions.data_ptr(),
-        positions.dtype == torch.int64, period, axes, freqs.data_ptr(), 2 * freqs.shape[0], interleaved, mscale,
-        out.data_ptr(), out.stride(0) if planes > 1 else 0, out.stride(1) if rows > 1 else 0, planes, rows, d,
-        x.dtype == torch.float16, _stream()), "samb_rotary")
+        x.data_ptr(), ps, rs, positions.data_ptr(), pt is torch.int64, period, axes, freqs.data_ptr(), 2 * freqs.shape[0],
+        interleaved, mscale, out.data_ptr(), ops_, ors, planes, rows, d, dtype is _F16, _stream()), "samb_rotary")
     return out
 
 
@@ -716,48 +754,76 @@ def route_topk(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] = None
     logits (plus ``bias [E]``, which decides the choice only; ties to the lower index), their softmax or sigmoid
     weights, and the order of the choices by expert for ``gemm_grouped`` and ``combine_topk``.  An expert at -inf or NaN
     is never chosen: a token with nobody left (a padded one) gets id -1, weight 0 and no place."""
-    _need(logits, torch.float32, "logits")
+    if logits.dtype is not _F32 or not logits.is_cuda:
+        _need(logits, _F32, "logits")
+    dev = torch.cuda.current_device()
+    _here(logits, _F32, dev, "logits")
     ld = _matrix(logits, "logits")
     T, E = logits.shape
     if not 1 <= k <= min(8, E):
         raise RuntimeError(f"k: {k} is not between 1 and 8 and at most the number of experts ({E})")
-    dev = logits.device
     lib = _lib.load()
     n = T * k
     scratch = lib.samb_route_scratch_bytes(T, E) // 4
     # one allocation for the whole numbers: ids, slots, rows, offsets, scratch
-    buf = torch.empty(3 * n + E + 1 + scratch, dtype=torch.int32, device=dev)
-    weights = torch.empty(T, k, dtype=torch.float32, device=dev)
+    buf = torch.empty((3 * n + E + 1 + scratch,), dtype=_I32, device=logits.device)
+    weights = torch.empty((T, k), dtype=_F32, device=logits.device)
     at = buf.data_ptr()
     _lib.check(lib.samb_route_topk(
-        logits.data_ptr(), ld, _vector(bias, "bias", E), T, E, k, sigmoid, renorm, scale, at, weights.data_ptr(),
-        at + 4 * n, at + 8 * n, at + 12 * n, at + 4 * (3 * n + E + 1), _stream()), "samb_route_topk")
+        logits.data_ptr(), ld, _vector(bias, "bias", dev, (E,)) if bias is not None else None, T, E, k, sigmoid, renorm,
+        scale, at, weights.data_ptr(), at + 4 * n, at + 8 * n, at + 12 * n, at + 4 * (3 * n + E + 1), _stream()),
+        "samb_route_topk")
     return Routing(buf.as_strided((T, k), (k, 1), 0), weights, buf.as_strided((T, k), (k, 1), n),
                    buf.as_strided((n,), (1,), 2 * n), buf.as_strided((E + 1,), (1,), 3 * n))
 
 
-def _grouped_args(a, w, offsets, rows, bias, out, out_dtype, kind):
+def _grouped(kind, a, a_scale, w, w_scale, offsets, rows, bias, gelu, out, dtype, dev):
+    int8 = dtype is torch.int8
+    odt = _BF16 if int8 else dtype
     lda = _matrix(a, "a")
-    if w.dim() != 3 or (w.shape[2] > 1 and w.stride(2) != 1):
-        raise RuntimeError("w: expected an [experts, N, K] tensor with unit inner stride")
+    _here(w, dtype, dev, "w")
+    if w.dim() != 3:
+        raise RuntimeError("w: expected an [experts, N, K] tensor")
     E, N, K = w.shape
-    if a.shape[1] != K:
+    ws, ldw, es = w.stride()
+    if es != 1 and K > 1:
+        raise RuntimeError("w: expected unit inner stride")
+    M, ka = a.shape
+    if ka != K:
         raise RuntimeError(f"{kind}: inner dimensions differ")
-    S = rows.shape[0] if rows is not None else a.shape[0]
+    lib = _lib.load()
+    prow = pbias = psc = None
+    S, epi = M, EPI_GELU if gelu else 0
+    if rows is not None:
+        S = rows.shape[0]
+        prow = _indexes(rows, "rows", dev, S)
+        room = lib.samb_gemm_grouped_scratch_bytes(S, E, K, int8)
+        if room:                                          # room to put the rows of a large product in order
+            scratch = torch.empty((room,), dtype=torch.uint8, device=a.device)
+            psc = scratch.data_ptr()
+    if bias is not None:
+        pbias = _vector(bias, "bias", dev, (E, N))
+        epi |= EPI_BIAS
+    poff = _indexes(offsets, "offsets", dev, E + 1)
     if out is None:
-        out = torch.empty(S, N, dtype=out_dtype, device=a.device)
+        out, ldo = torch.empty((S, N), dtype=odt, device=a.device), N
     else:
-        _need(out, out_dtype, "out")
-        if out.shape != (S, N):
-            raise RuntimeError(f"out: expected [{S}, {N}], got {list(out.shape)}")
-    scratch = None
-    if rows is not None:                                  # room to put the rows of a large product in order
-        n = _lib.load().samb_gemm_grouped_scratch_bytes(S, E, K, a.dtype == torch.int8)
-        if n:
-            scratch = torch.empty(n, dtype=torch.uint8, device=a.device)
-    return (scratch, lda, _indexes(rows, "rows", S) if rows is not None else None, w.stride(1) if N > 1 else K,
-            w.stride(0) if E > 1 else 0, _vector(bias, "bias", E, N), _indexes(offsets, "offsets", E + 1), out,
-            _matrix(out, "out"), S, E, N, K)
+        ldo = _like(out, odt, dev, (S, N), "out")
+    if N <= 1:
+        ldw = K
+    if E <= 1:
+        ws = 0
+    st = status_word(a.device).data_ptr()
+    if int8:
+        _lib.check(lib.samb_gemm_i8_grouped(
+            a.data_ptr(), lda, M, _vector(a_scale, "a_scale", dev, (M,)), prow, w.data_ptr(), ldw, ws,
+            _vector(w_scale, "w_scale", dev, (E, N)), pbias, poff, out.data_ptr(), ldo, S, E, N, K, epi, psc, st,
+            _stream()), "samb_gemm_i8_grouped")
+    else:
+        _lib.check(lib.samb_gemm_grouped(
+            a.data_ptr(), lda, M, prow, w.data_ptr(), ldw, ws, pbias, poff, out.data_ptr(), ldo, S, E, N, K,
+            dtype is _F16, epi, psc, st, _stream()), "samb_gemm_grouped")
+    return out
 
 
 def gemm_grouped(a: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows: Optional[torch.Tensor] = None,
@@ -767,14 +833,8 @@ def gemm_grouped(a: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows: 
     (without ``rows``: ``a[s]``), with ``a [M, K]`` and ``w [E, N, K]`` bfloat16 or float16, int32 ``offsets [E + 1]`` and
     ``rows [S]`` as ``route_topk`` gives them.  Rows of ``out [S, N]`` behind the last expert's are left as they were
     (unspecified in a new ``out``); an index outside ``a`` stands for a row of zeros."""
-    _need16(a, "a"); _need(w, a.dtype, "w")
-    scratch, lda, prow, ldw, ws, pbias, poff, out, ldo, S, E, N, K = _grouped_args(a, w, offsets, rows, bias, out,
-                                                                                  a.dtype, "gemm_grouped")
-    _lib.check(_lib.load().samb_gemm_grouped(
-        a.data_ptr(), lda, a.shape[0], prow, w.data_ptr(), ldw, ws, pbias, poff, out.data_ptr(), ldo, S, E, N, K,
-        a.dtype == torch.float16, (EPI_BIAS if bias is not None else 0) | (EPI_GELU if gelu else 0), _ptr(scratch),
-        status_word(a.device).data_ptr(), _stream()), "samb_gemm_grouped")
-    return out
+    dtype, dev = _half(a, "a")
+    return _grouped("gemm_grouped", a, None, w, None, offsets, rows, bias, gelu, out, dtype, dev)
 
 
 def gemm_i8_grouped(aq: torch.Tensor, a_scale: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor,
@@ -782,17 +842,11 @@ def gemm_i8_grouped(aq: torch.Tensor, a_scale: torch.Tensor, wq: torch.Tensor, w
                     gelu: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``gemm_grouped`` on int8 ``aq [M, K]`` with row scales ``a_scale [M]`` (gathered with the rows) and ``wq [E, N, K]``
     with ``w_scale [E, N]``: exact int32 accumulation, bf16 out."""
-    _need(aq, torch.int8, "aq"); _need(wq, torch.int8, "wq")
-    scratch, lda, prow, ldw, ws, pbias, poff, out, ldo, S, E, N, K = _grouped_args(aq, wq, offsets, rows, bias, out,
-                                                                                  torch.bfloat16, "gemm_i8_grouped")
+    _need(aq, torch.int8, "aq")
     if a_scale is None or w_scale is None:
         raise RuntimeError("gemm_i8_grouped needs both scales")
-    _lib.check(_lib.load().samb_gemm_i8_grouped(
-        aq.data_ptr(), lda, aq.shape[0], _vector(a_scale, "a_scale", aq.shape[0]), prow, wq.data_ptr(), ldw, ws,
-        _vector(w_scale, "w_scale", E, N), pbias, poff, out.data_ptr(), ldo, S, E, N, K,
-        (EPI_BIAS if bias is not None else 0) | (EPI_GELU if gelu else 0), _ptr(scratch),
-        status_word(aq.device).data_ptr(), _stream()), "samb_gemm_i8_grouped")
-    return out
+    return _grouped("gemm_i8_grouped", aq, a_scale, wq, w_scale, offsets, rows, bias, gelu, out, torch.int8,
+                    torch.cuda.current_device())
 
 
 def combine_topk(x: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, residual: Optional[torch.Tensor] = None,
@@ -800,28 +854,22 @@ def combine_topk(x: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, re
     """Weighted sum of the experts' rows back in token order: ``out[t] = residual[t] + sum_j weights[t, j] *
     x[slots[t, j]]`` with ``x [S, C]`` bfloat16 or float16, ``slots`` / ``weights`` ``[T, k]`` of ``route_topk`` (k up to 8);
     a slot of -1 adds nothing.  ``out`` may be ``residual``."""
-    _need16(x, "x")
+    dtype, dev = _half(x, "x")
     ldx = _matrix(x, "x")
     S, C = x.shape
-    if slots.dim() != 2:
-        raise RuntimeError("slots: expected a [T, k] tensor")
+    _here(slots, _I32, dev, "slots")
+    if slots.dim() != 2 or not slots.is_contiguous():
+        raise RuntimeError("slots: expected a contiguous [T, k] tensor")
     T, k = slots.shape
-    _need(slots, torch.int32, "slots")
-    if not slots.is_contiguous():
-        raise RuntimeError("slots must be contiguous")
-    ldr = 0
+    pr, ldr = None, 0
     if residual is not None:
-        _need(residual, x.dtype, "residual")
-        ldr = _matrix(residual, "residual")
-        if residual.shape != (T, C):
-            raise RuntimeError(f"residual: expected [{T}, {C}], got {list(residual.shape)}")
+        ldr = _like(residual, dtype, dev, (T, C), "residual")
+        pr = residual.data_ptr()
     if out is None:
-        out = torch.empty(T, C, dtype=x.dtype, device=x.device)
+        out, ldo = torch.empty((T, C), dtype=dtype, device=x.device), C
     else:
-        _need(out, x.dtype, "out")
-        if out.shape != (T, C):
-            raise RuntimeError(f"out: expected [{T}, {C}], got {list(out.shape)}")
+        ldo = _like(out, dtype, dev, (T, C), "out")
     _lib.check(_lib.load().samb_combine_topk(
-        x.data_ptr(), ldx, S, slots.data_ptr(), _vector(weights, "weights", T, k), _ptr(residual), ldr, out.data_ptr(),
-        _matrix(out, "out"), T, k, C, x.dtype == torch.float16, _stream()), "samb_combine_topk")
+        x.data_ptr(), ldx, S, slots.data_ptr(), _vector(weights, "weights", dev, (T, k)), pr, ldr, out.data_ptr(), ldo,
+        T, k, C, dtype is _F16, _stream()), "samb_combine_topk")
     return out
