@@ -403,7 +403,7 @@ __host__ __device__ constexpr int pair_smem_bytes(bool int8) {
 }
 __host__ __device__ constexpr int pair_threads(bool int8) { return 96 + 32 * pair_epi_warps(int8); }
 
-template <int kType, bool kGelu>
+template <int kType, bool kBias, bool kGelu>
 __global__ void __launch_bounds__(pair_threads(kType == kTypeI8), 1)
 grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmOut, const GroupedParams p) {
@@ -533,15 +533,15 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     }
   } else if (warp == 2 + kEpiWarps) {
     // ------------------------------------------------------------------ output warp
-    // Staged chunk n of this CTA lives in staging tile n % OUT_BUFS.  Only whole halves are staged.
+    // Staged chunk n of this CTA lives in staging tile n % OUT_BUFS.  Only whole tiles are staged.
     if (lane == 0) {
       uint32_t n = 0;
       bool ok = true;
       for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
         w.at(tile);
-        if (w.rows < skip + BM) continue;
         const int n0 = w.ntile * BN;
-        for (int c = 0; c < BN / 64 && n0 + c * 64 < p.N; ++c, ++n) {
+        if (w.rows < skip + BM || n0 + BN > p.N) continue;
+        for (int c = 0; c < BN / 64; ++c, ++n) {
           const uint32_t b = n % OUT_BUFS;
           if (!(ok = mbar_wait(&stage_full[b], (n / OUT_BUFS) & 1u, abort_flag, p.status, 6))) break;
           tma_store_2d(&tmOut, stage_out0 + b * OUT_STAGE_BYTES, n0 + c * 64, w.m0 + skip);
@@ -565,8 +565,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       w.at(tile);
       const int n0 = w.ntile * BN;
       const int mine = w.rows - skip;                    // rows of this CTA's half that exist (may be none)
-      const bool whole = mine >= BM;
-      const float* g_bias = p.bias != nullptr ? p.bias + (long long)w.e * p.N + n0 : nullptr;
+      const float* g_bias = kBias ? p.bias + (long long)w.e * p.N + n0 : nullptr;
       const float* g_wscale = kInt8 ? p.w_scale + (long long)w.e * p.N + n0 : nullptr;
       float a_scale = 1.f;
       if (kInt8 && erow < mine) {
@@ -576,41 +575,36 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[acc], acc_phase, abort_flag, p.status, 4))) break;
       tc_fence_after();
       const uint32_t t_addr = tmem_base + (lane_base << 16) + acc * BN + qc * CW;
-      // the tensor-memory load of chunk c + 1 is in flight while chunk c goes through the arithmetic, and the
-      // accumulator is handed back as soon as its last chunk is in registers
-      uint32_t rbuf[2][CW];
-      if constexpr (CW == 32) tmem_ld_32x32b_x32(t_addr, rbuf[0]);
-      else tmem_ld_32x32b_x16(t_addr, rbuf[0]);
+      if (mine >= BM && n0 + BN <= p.N) {
+        // A whole tile, without a branch in its arithmetic.  The tensor-memory load of chunk c + 1 is in flight while
+        // chunk c is worked on, and the accumulator is handed back as soon as its last chunk is in registers.
+        uint32_t rbuf[2][CW];
+        if constexpr (CW == 32) tmem_ld_32x32b_x32(t_addr, rbuf[0]);
+        else tmem_ld_32x32b_x16(t_addr, rbuf[0]);
 #pragma unroll
-      for (int c = 0; c < BN / 64; ++c) {
-        tmem_ld_wait();
-        if (c + 1 < BN / 64) {
-          if constexpr (CW == 32) tmem_ld_32x32b_x32(t_addr + (c + 1) * 64, rbuf[(c + 1) & 1]);
-          else tmem_ld_32x32b_x16(t_addr + (c + 1) * 64, rbuf[(c + 1) & 1]);
-        } else {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty0 + acc * 8);
-        }
-        if (n0 + c * 64 >= p.N || mine <= 0) continue;   // the same for the whole CTA
-        const uint32_t(&r)[CW] = rbuf[c & 1];
-        const uint32_t sbuf = chunk_no % OUT_BUFS, suse = chunk_no / OUT_BUFS;
-        uint8_t* stage_out = stage_out0 + sbuf * OUT_STAGE_BYTES;
-        bool ready = true;
-        if (whole && suse > 0) ready = mbar_test_wait(&stage_free[sbuf], (suse - 1u) & 1u);
-        uint4 packed[NV];
+        for (int c = 0; c < BN / 64; ++c) {
+          tmem_ld_wait();
+          if (c + 1 < BN / 64) {
+            if constexpr (CW == 32) tmem_ld_32x32b_x32(t_addr + (c + 1) * 64, rbuf[(c + 1) & 1]);
+            else tmem_ld_32x32b_x16(t_addr + (c + 1) * 64, rbuf[(c + 1) & 1]);
+          } else {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty0 + acc * 8);
+          }
+          const uint32_t(&r)[CW] = rbuf[c & 1];
+          const uint32_t sbuf = chunk_no % OUT_BUFS, suse = chunk_no / OUT_BUFS;
+          uint8_t* stage_out = stage_out0 + sbuf * OUT_STAGE_BYTES;
+          bool ready = true;
+          if (suse > 0) ready = mbar_test_wait(&stage_free[sbuf], (suse - 1u) & 1u);
+          uint4 packed[NV];
 #pragma unroll
-        for (int u = 0; u < NV; ++u) {
-          const int ct0 = c * 64 + qc * CW + u * 8;
-          packed[u] = make_uint4(0u, 0u, 0u, 0u);
-          if (n0 + ct0 < p.N) {                          // N is a multiple of 8
+          for (int u = 0; u < NV; ++u) {
+            const int ct0 = c * 64 + qc * CW + u * 8;
             float v[8];
-            if (g_bias != nullptr) epilogue8<kInt8, kInt8, true, kGelu>(r + u * 8, a_scale, g_wscale + ct0, g_bias + ct0, v);
-            else epilogue8<kInt8, kInt8, false, kGelu>(r + u * 8, a_scale, g_wscale + ct0, nullptr, v);
+            epilogue8<kInt8, kInt8, kBias, kGelu>(r + u * 8, a_scale, g_wscale + ct0, g_bias + ct0, v);
             packed[u] = kType == kTypeF16 ? F16::pack(v) : Bf16::pack(v);
           }
-        }
-        if (whole) {
           if (!ready) mbar_wait(&stage_free[sbuf], (suse - 1u) & 1u, abort_flag, p.status, 7);
           uint8_t* srow = stage_out + erow * 128;
 #pragma unroll
@@ -620,15 +614,30 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           __syncwarp();
           if (lane == 0) mbar_arrive(&stage_full[sbuf]);
           ++chunk_no;
-        } else if (erow < mine) {
-          // the last rows of an expert: straight from registers (one tile in many)
+        }
+      } else {
+        // The last rows of an expert or the last columns: straight from registers (N is a multiple of 8).
+#pragma unroll 1
+        for (int c = 0; c < BN / 64 && n0 + c * 64 < p.N && mine > 0; ++c) {
+          uint32_t r[CW];
+          if constexpr (CW == 32) tmem_ld_32x32b_x32(t_addr + c * 64, r);
+          else tmem_ld_32x32b_x16(t_addr + c * 64, r);
+          tmem_ld_wait();
           uint16_t* o = static_cast<uint16_t*>(p.out) + (w.m0 + skip + (long long)erow) * p.ldo + n0;
 #pragma unroll
           for (int u = 0; u < NV; ++u) {
             const int ct0 = c * 64 + qc * CW + u * 8;
-            if (n0 + ct0 < p.N) *reinterpret_cast<uint4*>(o + ct0) = packed[u];
+            if (n0 + ct0 < p.N && erow < mine) {
+              float v[8];
+              epilogue8<kInt8, kInt8, kBias, kGelu>(r + u * 8, a_scale, g_wscale + ct0, g_bias + ct0, v);
+              *reinterpret_cast<uint4*>(o + ct0) = kType == kTypeF16 ? F16::pack(v) : Bf16::pack(v);
+            }
           }
+          __syncwarp();
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty0 + acc * 8);
       }
       if (++acc == NUM_ACC) { acc = 0; acc_phase ^= 1u; }
     }
@@ -846,10 +855,13 @@ GroupedFn one_of(bool gelu, bool gather) {
 GroupedFn one_kernel(int type, bool gelu, bool gather) {
   return type == kTypeBf16 ? one_of<kTypeBf16>(gelu, gather) : type == kTypeF16 ? one_of<kTypeF16>(gelu, gather) : one_of<kTypeI8>(gelu, gather);
 }
-GroupedFn pair_kernel(int type, bool gelu) {
-  if (type == kTypeBf16) return gelu ? grouped_pair_kernel<kTypeBf16, true> : grouped_pair_kernel<kTypeBf16, false>;
-  if (type == kTypeF16) return gelu ? grouped_pair_kernel<kTypeF16, true> : grouped_pair_kernel<kTypeF16, false>;
-  return gelu ? grouped_pair_kernel<kTypeI8, true> : grouped_pair_kernel<kTypeI8, false>;
+template <int kType>
+GroupedFn pair_of(bool bias, bool gelu) {
+  if (bias) return gelu ? grouped_pair_kernel<kType, true, true> : grouped_pair_kernel<kType, true, false>;
+  return gelu ? grouped_pair_kernel<kType, false, true> : grouped_pair_kernel<kType, false, false>;
+}
+GroupedFn pair_kernel(int type, bool bias, bool gelu) {
+  return type == kTypeBf16 ? pair_of<kTypeBf16>(bias, gelu) : type == kTypeF16 ? pair_of<kTypeF16>(bias, gelu) : pair_of<kTypeI8>(bias, gelu);
 }
 
 // Rows per expert from which the pair kernel is the faster one.
@@ -860,7 +872,8 @@ bool want_pairs(int64_t S, int E) { return S >= kPairRows * int64_t(E); }
 int launch_pairs(int type, bool gelu, const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmOut,
                  const GroupedParams& p, void* scratch, cudaStream_t st) {
   const bool int8 = type == kTypeI8;
-  const GroupedFn kern = pair_kernel(type, gelu);
+  const bool bias = p.bias != nullptr;
+  const GroupedFn kern = pair_kernel(type, bias, gelu);
   const int smem_bytes = pair_smem_bytes(int8);
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes) != cudaSuccess) return SAMB_E_LAUNCH;
   cudaLaunchConfig_t cfg = {};
@@ -875,8 +888,8 @@ int launch_pairs(int type, bool gelu, const CUtensorMap& tmA, const CUtensorMap&
   cfg.dynamicSmemBytes = size_t(smem_bytes);
   cfg.stream = st;
   cfg.gridDim = dim3(unsigned(sm_count() & ~1));
-  static int cached_clusters[3][2] = {};                  // co-resident pairs per kernel variant (0 = not asked yet)
-  int& max_clusters = cached_clusters[type][gelu ? 1 : 0];
+  static int cached_clusters[3][4] = {};                  // co-resident pairs per kernel variant (0 = not asked yet)
+  int& max_clusters = cached_clusters[type][(bias ? 2 : 0) + (gelu ? 1 : 0)];
   if (max_clusters == 0 &&
       (cudaOccupancyMaxActiveClusters(&max_clusters, kern, &cfg) != cudaSuccess || max_clusters < 1)) {
     cudaGetLastError();
