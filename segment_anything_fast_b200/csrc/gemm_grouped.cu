@@ -14,8 +14,9 @@
 // against 590 us for rows in order at 65536 x 5120 x 1280; TMA's own gather of four rows, at some 85 cycles an
 // instruction, took 2110 us), so its rows are put in order first, in caller scratch: a pass at copy bandwidth (30 us).
 //
-// A tile computes all its rows whatever its expert has left, but stores only its own: whole 128-row halves leave by
-// TMA, the last ones of an expert row by row.
+// A tile computes all its rows whatever its expert has left (the rows behind them in shared memory may be anything: a
+// row of the product depends on its own row of A alone), but stores only its own: whole tiles leave by TMA, the last
+// ones of an expert row by row.
 #include "elem16.cuh"
 
 namespace samb {
@@ -107,7 +108,7 @@ struct TileWalk {
 
 // A gathering warp owns one stage of the ring: for every STAGES-th slab it waits until the stage is free, fetches 128
 // rows of A (from row `skip` of the tile) with 32 cp.async a lane, eight lanes a row, waits for them and passes the slab
-// on.  Rows and columns that do not exist are filled with zeros.  cp.async writes through the generic proxy and the
+// on.  Rows whose index lies outside A and columns behind K are filled with zeros.  cp.async writes through the generic proxy and the
 // tensor core reads through the async one; the fence between the two waits for the thread's copies in flight, so a
 // thread with several slabs in flight would pay the whole memory latency for each of them.  Here the warps overlap.
 template <int STAGES, int kStageBytes, typename Arrive>
@@ -138,6 +139,7 @@ __device__ __forceinline__ void gather_role(const GroupedParams& p, TileWalk w, 
       const uint8_t* base = p.a + (inside ? k0 : 0);
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
+        if (j * 4 >= w.rows - skip) break;               // what lies behind the tile's rows may be anything
         const int r = __shfl_sync(0xffffffffu, idx[j >> 3], (j & 7) * 4 + quarter);
         const bool there = inside && r >= 0;
         const uint8_t* s = base + (there ? r : 0) * p.a_pitch;
@@ -176,15 +178,15 @@ __device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, 256;" :::
 // ---------------------------------------------------------------------------------------------- single CTAs
 constexpr int ONE_STAGES = 4;
 constexpr int ONE_STAGE_BYTES = A_STAGE_BYTES + BN * SLAB_BYTES;
-constexpr int B_BOX_ROWS = 64;
-constexpr int B_BOX_BYTES = B_BOX_ROWS * SLAB_BYTES;
+constexpr int A_BOX_ROWS = 32;                           // up to 64 rows of A: only the boxes that hold some are loaded
+constexpr int A_BOX_BYTES = A_BOX_ROWS * SLAB_BYTES;
 constexpr int ONE_THREADS = 64 + 256;                    // producer, MMA, eight epilogue warps (and the gathering ones)
 constexpr int ONE_SMEM_BYTES = ONE_STAGES * ONE_STAGE_BYTES + OUT_STAGE_BYTES + 2 * BN * 4 + 2 * (kMaxExperts + 1) * 4 + 1024 + 256;
 
 template <int kType, bool kGelu, bool kGather>
 __global__ void __launch_bounds__(ONE_THREADS + (kGather ? 32 * ONE_STAGES : 0), 1)
-grouped_one_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                   const __grid_constant__ CUtensorMap tmOut, const GroupedParams p) {
+grouped_one_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA32,
+                   const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmOut, const GroupedParams p) {
   constexpr bool kInt8 = kType == kTypeI8;
   constexpr int STAGES = ONE_STAGES, STAGE_BYTES = ONE_STAGE_BYTES;
   extern __shared__ uint8_t smem_raw[];
@@ -216,7 +218,10 @@ grouped_one_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       mbar_init(&acc_empty[a], 8);
     }
     fence_mbar_init();
-    if (!kGather) tma_prefetch_desc(&tmA);
+    if (!kGather) {
+      tma_prefetch_desc(&tmA);
+      tma_prefetch_desc(&tmA32);
+    }
     tma_prefetch_desc(&tmB);
     tma_prefetch_desc(&tmOut);
   }
@@ -227,11 +232,14 @@ grouped_one_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   if (warp == 2) {
     const int tiles = tile_list(p, BM, s_first, s_start);
     if (lane == 0) {
-      // column tile: waves x (columns + what a tile costs beside its columns), so that the last wave is not mostly empty
-      int best = 0, bn = BN;
-      for (int w = BN; w >= 64; w >>= 1) {
+      // Column tile: waves x what a tile takes, in columns a K step: its own, as much as 64 more for its rows, and some 1000
+      // in all for its start and epilogue.  A last wave that is mostly empty makes narrower tiles the better ones (3072
+      // rows of 16 experts, 1280 x 5120: 192 columns 70 us, 256 columns 87 us).
+      long long best = 0;
+      int bn = BN;
+      for (int w = BN; w >= 64; w -= 64) {
         const long long t = (long long)tiles * ((p.N + w - 1) / w);
-        const int cost = int((t + gridDim.x - 1) / gridDim.x) * (w + 64);
+        const long long cost = ((t + gridDim.x - 1) / gridDim.x) * ((long long)p.k_slabs * (w + 64) + 1000);
         if (w == BN || cost < best) { best = cost; bn = w; }
       }
       *s_bn = bn;
@@ -255,17 +263,24 @@ grouped_one_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
       w.at(tile);
       const int n0 = w.ntile * bn;
+      const int a_boxes = w.rows > 2 * A_BOX_ROWS ? BM / A_BOX_ROWS : (w.rows + A_BOX_ROWS - 1) / A_BOX_ROWS;
       for (int ks = 0; ks < p.k_slabs; ++ks) {
         if (!(ok = __all_sync(0xffffffffu, mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, 1)))) break;
         uint8_t* sa = smem + stage * STAGE_BYTES;
-        if (lane == 0) {
-          mbar_expect_tx(&full_bar[stage], (kGather ? 0 : A_STAGE_BYTES) + bn * SLAB_BYTES);
-          if (!kGather) tma_load_2d(sa, &tmA, &full_bar[stage], ks * slab_elems, w.m0);
+        uint64_t* bar = &full_bar[stage];
+        if (lane == 0) mbar_expect_tx(bar, (kGather ? 0 : a_boxes * A_BOX_BYTES) + bn * SLAB_BYTES);
+        __syncwarp();
+        // W in pieces of 64 rows
+        if (!kGather) {
+          if (a_boxes == BM / A_BOX_ROWS) {
+            if (lane == 0) tma_load_2d(sa, &tmA, bar, ks * slab_elems, w.m0);
+          } else if (lane >= 8 && lane < 8 + a_boxes) {
+            tma_load_2d(sa + (lane - 8) * A_BOX_BYTES, &tmA32, bar, ks * slab_elems, w.m0 + (lane - 8) * A_BOX_ROWS);
+          }
         }
         __syncwarp();
-        if (lane < bn / B_BOX_ROWS)
-          tma_load_3d(sa + A_STAGE_BYTES + lane * B_BOX_BYTES, &tmB, &full_bar[stage], ks * slab_elems,
-                      n0 + lane * B_BOX_ROWS, w.e);
+        if (lane < bn / 64)
+          tma_load_3d(sa + A_STAGE_BYTES + lane * (64 * SLAB_BYTES), &tmB, bar, ks * slab_elems, n0 + lane * 64, w.e);
         ++issued;
         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
       }
@@ -328,7 +343,7 @@ grouped_one_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       }
       float a_scale = 1.f;
       if (kInt8 && erow < w.rows) {
-        const int i = kGather ? __ldg(p.rows + w.m0 + erow) : w.m0 + erow;
+        const int i = p.rows != nullptr ? __ldg(p.rows + w.m0 + erow) : w.m0 + erow;
         if (i >= 0 && i < p.a_rows) a_scale = __ldg(p.a_scale + i);        // else: a row of zeros, whatever its scale
       }
       const bool got = mbar_wait(&acc_full[acc], acc_phase, abort_flag, p.status, 4);
@@ -845,35 +860,41 @@ order_rows_kernel(const GroupedParams p, uint4* __restrict__ to) {
     if (i0 + u * 256 < last) to[i0 + u * 256] = v[u];
 }
 
-using GroupedFn = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const GroupedParams);
+using PairFn = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const GroupedParams);
+using OneFn = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const CUtensorMap, const GroupedParams);
 
 template <int kType>
-GroupedFn one_of(bool gelu, bool gather) {
+OneFn one_of(bool gelu, bool gather) {
   if (gelu) return gather ? grouped_one_kernel<kType, true, true> : grouped_one_kernel<kType, true, false>;
   return gather ? grouped_one_kernel<kType, false, true> : grouped_one_kernel<kType, false, false>;
 }
-GroupedFn one_kernel(int type, bool gelu, bool gather) {
+OneFn one_kernel(int type, bool gelu, bool gather) {
   return type == kTypeBf16 ? one_of<kTypeBf16>(gelu, gather) : type == kTypeF16 ? one_of<kTypeF16>(gelu, gather) : one_of<kTypeI8>(gelu, gather);
 }
 template <int kType>
-GroupedFn pair_of(bool bias, bool gelu) {
+PairFn pair_of(bool bias, bool gelu) {
   if (bias) return gelu ? grouped_pair_kernel<kType, true, true> : grouped_pair_kernel<kType, true, false>;
   return gelu ? grouped_pair_kernel<kType, false, true> : grouped_pair_kernel<kType, false, false>;
 }
-GroupedFn pair_kernel(int type, bool bias, bool gelu) {
+PairFn pair_kernel(int type, bool bias, bool gelu) {
   return type == kTypeBf16 ? pair_of<kTypeBf16>(bias, gelu) : type == kTypeF16 ? pair_of<kTypeF16>(bias, gelu) : pair_of<kTypeI8>(bias, gelu);
 }
 
-// Rows per expert from which the pair kernel is the faster one.
-constexpr int64_t kPairRows = 192;
-
+// Pairs from 512 rows an expert.  16 experts, us, single CTAs against pairs: 5120 x 1280 bf16: 70 / 73 at 256 rows, 91 / 92
+// at 384, 112 / 103 at 512; 1280 x 5120: 74 / 70, 86 / 94, 114 / 107; 5120 x 1280 int8: 39 / 42, 47 / 49, 57 / 58.
+constexpr int64_t kPairRows = 512;
 bool want_pairs(int64_t S, int E) { return S >= kPairRows * int64_t(E); }
 
+// Gathered rows are put in order first from 32 rows an expert, when a row has 1 KB at least (16 experts, 5120 x 1280 bf16,
+// in the kernel against a pass first: 41 / 41 us at 16 rows an expert, 46 / 42 at 32, 56 / 48 at 64, 69 / 48 at 128; 64
+// experts, 512 x 256: 10.9 / 12.3 at 16, 15.1 / 15.8 at 128), and always for pairs.
+bool want_order(int64_t S, int E, int64_t row_bytes) { return want_pairs(S, E) || (S >= 32 * int64_t(E) && row_bytes >= 1024); }
+
 int launch_pairs(int type, bool gelu, const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmOut,
-                 const GroupedParams& p, void* scratch, cudaStream_t st) {
+                 const GroupedParams& p, cudaStream_t st) {
   const bool int8 = type == kTypeI8;
   const bool bias = p.bias != nullptr;
-  const GroupedFn kern = pair_kernel(type, bias, gelu);
+  const PairFn kern = pair_kernel(type, bias, gelu);
   const int smem_bytes = pair_smem_bytes(int8);
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes) != cudaSuccess) return SAMB_E_LAUNCH;
   cudaLaunchConfig_t cfg = {};
@@ -896,12 +917,6 @@ int launch_pairs(int type, bool gelu, const CUtensorMap& tmA, const CUtensorMap&
     max_clusters = -1;
   }
   if (max_clusters < 1) return SAMB_E_SHAPE;
-  if (p.rows != nullptr) {
-    const long long vecs = p.S * (p.k_bytes / 16);
-    const long long blocks = (vecs + 256 * kOrderVecs - 1) / (256 * kOrderVecs);
-    order_rows_kernel<<<unsigned(blocks), 256, 0, st>>>(p, static_cast<uint4*>(scratch));
-    if (int e = launch_status()) return e;
-  }
   long long pairs = max_clusters < sm_count() / 2 ? max_clusters : sm_count() / 2;
   const long long most = ((p.S + 2 * BM - 1) / (2 * BM) + p.E) * ((p.N + BN - 1) / BN);
   if (most < pairs) pairs = most;
@@ -941,14 +956,13 @@ int launch_grouped(int type, const void* A, int64_t lda, int64_t a_rows, const f
   const CUtensorMapDataType dt = type == kTypeI8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                  : type == kTypeF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const uint32_t slab_elems = uint32_t(SLAB_BYTES / esz);
-  CUtensorMap tmA, tmB, tmOut;
-  auto map_a = [&](const void* base, int64_t ld, int64_t n) {
+  CUtensorMap tmA, tmA32, tmB, tmOut;
+  auto map_a = [&](CUtensorMap* to, const void* base, int64_t ld, int64_t n, int box_rows) {
     const uint64_t dims[2] = {uint64_t(K), uint64_t(n)};
     const uint64_t strides[2] = {uint64_t(esz), uint64_t(ld) * esz};
-    const uint32_t box[2] = {slab_elems, uint32_t(BM)};
-    return make_tensor_map(&tmA, dt, 2, const_cast<void*>(base), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    const uint32_t box[2] = {slab_elems, uint32_t(box_rows)};
+    return make_tensor_map(to, dt, 2, const_cast<void*>(base), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
   };
-  // W in boxes of half a pair's column tile, or of the narrowest single-CTA one
   auto map_w = [&](int box_rows) {
     const uint64_t dims[3] = {uint64_t(K), uint64_t(N), uint64_t(E)};
     const uint64_t strides[3] = {uint64_t(esz), uint64_t(ldw) * esz, uint64_t(E > 1 ? w_stride : ldw * N) * esz};
@@ -980,22 +994,33 @@ int launch_grouped(int type, const void* A, int64_t lda, int64_t a_rows, const f
     else launch_few<kTypeI8>(w, pitch, stride, p, gelu, st);
     return launch_status();
   }
+  // what the products read: A itself, or its rows in order in the caller's scratch
+  const bool order = gather && scratch != nullptr && want_order(S, E, p.k_bytes);
+  const void* from = order ? scratch : A;
+  const int64_t from_ld = order ? K : lda, from_rows = order ? S : a_rows;
+  if (order) {
+    const long long vecs = S * (p.k_bytes / 16), blocks = (vecs + 256 * kOrderVecs - 1) / (256 * kOrderVecs);
+    if (blocks > 0x7fffffff) return SAMB_E_SHAPE;
+    order_rows_kernel<<<unsigned(blocks), 256, 0, st>>>(p, static_cast<uint4*>(scratch));
+    if (int e = launch_status()) return e;
+  }
+  if (int e = map_a(&tmA, from, from_ld, from_rows, BM)) return e;
   // the pair kernel's epilogue reads the column vectors in 16-byte pieces; it wants its rows in order
-  if (want_pairs(S, E) && (!gather || scratch != nullptr) &&
+  if (want_pairs(S, E) && (!gather || order) &&
       !((reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(w_scale)) & 15u)) {
-    if (int e = gather ? map_a(scratch, K, S) : map_a(A, lda, a_rows)) return e;
     if (int e = map_w(BN / 2)) return e;
-    const int e = launch_pairs(type, gelu, tmA, tmB, tmOut, p, scratch, st);
+    const int e = launch_pairs(type, gelu, tmA, tmB, tmOut, p, st);
     if (e != SAMB_E_SHAPE) return e;                     // pairs cannot be placed on this GPU: single CTAs
   }
-  if (int e = map_a(A, lda, a_rows)) return e;
-  if (int e = map_w(B_BOX_ROWS)) return e;
-  const GroupedFn kern = one_kernel(type, gelu, gather);
+  if (int e = map_a(&tmA32, from, from_ld, from_rows, A_BOX_ROWS)) return e;
+  if (int e = map_w(64)) return e;
+  const bool in_kernel = gather && !order;
+  const OneFn kern = one_kernel(type, gelu, in_kernel);
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ONE_SMEM_BYTES) != cudaSuccess)
     return SAMB_E_LAUNCH;
   const long long most = ((S + BM - 1) / BM + E) * ((N + 63) / 64);
   const unsigned grid = unsigned(most < sm_count() ? most : sm_count());
-  kern<<<grid, ONE_THREADS + (gather ? 32 * ONE_STAGES : 0), ONE_SMEM_BYTES, st>>>(tmA, tmB, tmOut, p);
+  kern<<<grid, ONE_THREADS + (in_kernel ? 32 * ONE_STAGES : 0), ONE_SMEM_BYTES, st>>>(tmA, tmA32, tmB, tmOut, p);
   return launch_status();
 }
 
@@ -1005,8 +1030,8 @@ int launch_grouped(int type, const void* A, int64_t lda, int64_t a_rows, const f
 extern "C" {
 
 int64_t samb_gemm_grouped_scratch_bytes(int64_t S, int E, int K, int is_i8) {
-  if (S <= 0 || E <= 0 || K <= 0 || !samb::want_pairs(S, E)) return 0;
-  return S * K * (is_i8 ? 1 : 2);
+  const int64_t row = int64_t(K) * (is_i8 ? 1 : 2);
+  return S > samb::kFewSlots && E > 0 && K > 0 && samb::want_order(S, E, row) ? S * row : 0;
 }
 
 int samb_gemm_grouped(const void* A, int64_t lda, int64_t a_rows, const int32_t* rows, const void* W, int64_t ldw,

@@ -378,7 +378,8 @@ CASES = [  # counts of the experts, rows behind the last, N, K, padded strides
     ([1], 0, 8, 16, 0), ([1, 1], 0, 256, 64, 0), ([0, 2, 0, 1, 0], 3, 264, 80, 0), ([127, 128, 129], 0, 256, 320, 0),
     ([0, 0, 300, 0], 5, 520, 64, 0), ([5, 260, 1, 0, 64], 0, 72, 144, 1), ([1] * 33, 2, 64, 96, 0), ([3] * 300, 0, 40, 32, 0),
     ([700, 11, 90], 0, 1280, 1280, 0), ([1] * 8, 0, 1280, 5120, 0), ([8, 0, 3], 1, 640, 1296, 1), ([2] * 16, 0, 2560, 256, 0),
-    ([4000, 3000, 1192], 0, 512, 128, 0)]
+    ([4000, 3000, 1192], 0, 512, 128, 0), ([1500, 3, 257], 0, 520, 144, 1), ([2000, 0], 7, 264, 80, 0), ([600], 0, 8, 16, 0),
+    ([100, 40, 0, 200], 0, 256, 1040, 0)]
 
 
 @pytest.mark.parametrize("t", [BF16, F16, torch.int8])
@@ -430,10 +431,10 @@ def test_gemm_grouped_without_scratch_and_with_an_odd_bias(ops, t):
     """A product large enough for CTA pairs whose caller has no scratch, or whose bias starts at an odd place."""
     from segment_anything_fast_b200 import _lib
     g = gen(12)
-    S, M, E, N, K = 1500, 700, 3, 264, 160
+    S, M, E, N, K = 1700, 700, 3, 264, 160
     a, w, sa, sw = operands(g, t, M, E, N, K)
     rows = torch.randint(0, M, (S,), generator=g, device="cuda", dtype=torch.int32)
-    off = torch.tensor([0, 400, 1200, 1490], dtype=torch.int32, device="cuda")
+    off = torch.tensor([0, 400, 1200, 1690], dtype=torch.int32, device="cuda")
     bias = rand(g, E * N + 1)[1:].reshape(E, N)
     want, slack, written = grouped64(a, w, off, rows, bias, True, S, sa, sw)
     got = call_grouped(ops, a, w, sa, sw, off, rows=rows, bias=bias, gelu=True)
