@@ -11,7 +11,7 @@
 // Its top 32 bits are the argument of sincospi: the angle is off by 2^-32 turns and position * 2^-64 turns.
 //
 // A thread owns V pairs of a position and walks over the copies that share it (planes x repetitions of the
-// positions), so the angles are worked out once and the copies stream.
+// positions), so the angles are worked out once and the copies stream, four of them in flight a thread.
 #include "elem16.cuh"
 
 namespace samb {
@@ -26,6 +26,7 @@ struct RotaryParams {
   unsigned period;                 // positions
   unsigned repeats;                // rows = repeats * period
   unsigned planes;
+  unsigned step_plane, step_rep;   // gridDim.y copies on: so many planes and repetitions
   int pos64, axes, rot, half, d;
   int units, tails, tail_len;      // V-pair units of a row, then units of tail_len copied elements
   float mscale;
@@ -61,13 +62,22 @@ rotary_kernel(const RotaryParams p) {
   const unsigned row = unsigned(t / per_row);
   const int u = int(t - (unsigned long long)row * per_row);
   if (row >= p.period) return;
-  const unsigned copies = p.planes * p.repeats;
-  const bool tail = u >= p.units;
+  // the copies of this thread: blockIdx.y, blockIdx.y + gridDim.y, ..., as (plane, repetition)
+  unsigned left = (p.planes * p.repeats - blockIdx.y + gridDim.y - 1) / gridDim.y;
+  unsigned plane = blockIdx.y / p.repeats, rep = blockIdx.y - plane * p.repeats;
+  auto next = [&]() {
+    plane += p.step_plane;
+    rep += p.step_rep;
+    if (rep >= p.repeats) {
+      rep -= p.repeats;
+      ++plane;
+    }
+  };
 
-  if (tail) {
+  if (u >= p.units) {                                    // elements behind the rotated ones
     const int c = p.rot + (u - p.units) * p.tail_len;
-    for (unsigned i = blockIdx.y; i < copies; i += gridDim.y) {
-      const unsigned plane = i / p.repeats, r = (i - plane * p.repeats) * p.period + row;
+    for (; left > 0; --left, next()) {
+      const long long r = (long long)rep * p.period + row;
       const uint16_t* src = p.x + plane * p.xp + r * p.xr + c;
       uint16_t* dst = p.out + plane * p.op + r * p.orow + c;
       if (p.tail_len == 8) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
@@ -93,34 +103,38 @@ rotary_kernel(const RotaryParams p) {
     sn[j] *= p.mscale;
   }
 
-#pragma unroll 4
-  for (unsigned i = blockIdx.y; i < copies; i += gridDim.y) {
-    const unsigned plane = i / p.repeats, r = (i - plane * p.repeats) * p.period + row;
-    const uint16_t* src = p.x + plane * p.xp + r * p.xr;
-    uint16_t* dst = p.out + plane * p.op + r * p.orow;
-    if (kInter) {
-      alignas(16) uint16_t e[2 * V], o[2 * V];
-      load_vec<2 * V>(src + u * 2 * V, e);
+  // the two parts of the unit: neighbours are one run of 2 V elements, halves are two runs of V
+  constexpr int kRun = kInter ? 2 * V : V, kRuns = kInter ? 1 : 2;
+  const int c = u * kRun;
+  while (left > 0) {
+    alignas(16) uint16_t e[4][kRuns][kRun];
+    uint16_t* dst[4];
+    const unsigned n = min(left, 4u);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float a = T::to_float(e[2 * j]), b = T::to_float(e[2 * j + 1]);
-        o[2 * j] = T::from_float(fmaf(a, cs[j], -b * sn[j]));
-        o[2 * j + 1] = T::from_float(fmaf(b, cs[j], a * sn[j]));
-      }
-      store_vec<2 * V>(dst + u * 2 * V, o);
-    } else {
-      alignas(16) uint16_t e0[V], e1[V], o0[V], o1[V];
-      load_vec<V>(src + u * V, e0);
-      load_vec<V>(src + p.half + u * V, e1);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float a = T::to_float(e0[j]), b = T::to_float(e1[j]);
-        o0[j] = T::from_float(fmaf(a, cs[j], -b * sn[j]));
-        o1[j] = T::from_float(fmaf(b, cs[j], a * sn[j]));
-      }
-      store_vec<V>(dst + u * V, o0);
-      store_vec<V>(dst + p.half + u * V, o1);
+    for (int b = 0; b < 4; ++b) {
+      if (b >= n) break;
+      const long long r = (long long)rep * p.period + row;
+      const uint16_t* src = p.x + plane * p.xp + r * p.xr + c;
+      dst[b] = p.out + plane * p.op + r * p.orow + c;
+      load_vec<kRun>(src, e[b][0]);
+      if (!kInter) load_vec<kRun>(src + p.half, e[b][kRuns - 1]);
+      next();
     }
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      if (b >= n) break;
+      alignas(16) uint16_t o[kRuns][kRun];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int r1 = kRuns - 1, j0 = kInter ? 2 * j : j, j1 = kInter ? 2 * j + 1 : j;
+        const float a = T::to_float(e[b][0][j0]), d = T::to_float(e[b][r1][j1]);
+        o[0][j0] = T::from_float(fmaf(a, cs[j], -d * sn[j]));
+        o[r1][j1] = T::from_float(fmaf(d, cs[j], a * sn[j]));
+      }
+      store_vec<kRun>(dst[b], o[0]);
+      if (!kInter) store_vec<kRun>(dst[b] + p.half, o[kRuns - 1]);
+    }
+    left -= n;
   }
 }
 
@@ -135,6 +149,8 @@ int launch_rotary(RotaryParams p, cudaStream_t st) {
   unsigned long long by = ((unsigned long long)sm_count() * 8 + bx - 1) / bx;
   if (by > copies) by = copies;
   if (by > 65535) by = 65535;
+  p.step_plane = unsigned(by) / p.repeats;
+  p.step_rep = unsigned(by) % p.repeats;
   rotary_kernel<T, kInter, V><<<dim3(unsigned(bx), unsigned(by)), 256, 0, st>>>(p);
   return launch_status();
 }

@@ -1,12 +1,12 @@
 // The router of a mixture of experts: every token's k largest logits, their weights, and the order of the chosen
 // (token, choice) pairs by expert in which the grouped products take them.
 //
-// Choice: a warp holds a token's logits (up to 512, 16 a lane) as order-preserving integers; each of the k rounds is
-// a warp maximum and a warp minimum of the indexes that reach it, so ties go to the lowest index.  Order: a stable
-// counting sort.  Each block counts the experts of its own run of tokens; then (second launch, or after a barrier when
-// one block is enough) it adds up the counts of the blocks before it and places its pairs in order: a warp owns a run
-// of pairs, ranks equal experts among its lanes with match_any and keeps a running count per expert in shared
-// memory.  Nothing depends on the order in which atomics arrive.
+// Choice: eight lanes (up to 64 experts: four tokens a warp) or a warp (up to 512) hold a token's logits as order-preserving
+// integers, the next tokens' on their way; each of the k rounds is a maximum over the lanes, the lowest index among
+// equals.  Order: a stable counting sort.  Each block counts the experts of its own run of tokens; then (second launch, or
+// after a barrier when one block is enough) it adds up the counts of the blocks before it and places its pairs in
+// order: a warp owns a run of pairs, ranks equal experts among its lanes with match_any and keeps a running count per
+// expert in shared memory.  Nothing depends on the order in which atomics arrive.
 #include "common.cuh"
 
 namespace samb {
@@ -41,89 +41,131 @@ __device__ __forceinline__ unsigned order_key(float v) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-template <int NE>
-__device__ __forceinline__ void choose_token(const RouteParams& p, int token, int lane) {
+// L lanes a token (8 or 32); lane `sub` of them holds the experts i * L + sub.
+template <int L, int NE>
+__device__ __forceinline__ void load_logits(const RouteParams& p, int token, bool live, float (&x)[NE]) {
+  const int sub = threadIdx.x & (L - 1);
   const float* lr = p.logits + token * p.ld;
-  float v[NE];
-  unsigned key[NE];
-  float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < NE; ++i) {
-    const int e = i * 32 + lane;
-    v[i] = -INFINITY;
-    key[i] = 0u;
-    if (e < p.E) {
-      const float x = __ldg(lr + e);
-      key[i] = order_key(p.bias != nullptr ? x + __ldg(p.bias + e) : x);
-      if (x > -INFINITY) v[i] = fminf(x, 3.402823466e38f);
-      else key[i] = 0u;                                  // switched off, whatever the bias says
-    }
-    top = fmaxf(top, v[i]);
+    const int e = i * L + sub;
+    x[i] = live && e < p.E ? __ldg(lr + e) : -INFINITY;
   }
-  float denom = 1.f;
-  if (!p.sigmoid && !p.renorm) {                         // the sum over all experts cancels when renormalising
+}
+
+template <int L>
+__device__ __forceinline__ float lanes_max(float v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  for (int o = L / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <int L, int NE>
+__device__ __forceinline__ void choose_token(const RouteParams& p, int token, bool live, const float (&bias)[NE],
+                                             const float (&x)[NE]) {
+  const int lane = threadIdx.x & 31, sub = lane & (L - 1);
+  float v[NE];
+  unsigned key[NE];
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    const bool on = x[i] > -INFINITY;                    // neither switched off (whatever the bias says) nor NaN
+    v[i] = on ? fminf(x[i], 3.402823466e38f) : -INFINITY;
+    key[i] = on ? order_key(p.bias != nullptr ? x[i] + bias[i] : x[i]) : 0u;
+  }
+  float top = 0.f, denom = 1.f;
+  if (!p.sigmoid && !p.renorm) {                         // the sum over all experts cancels when renormalising
+    top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) top = fmaxf(top, v[i]);
+    top = lanes_max<L>(top);
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < NE; ++i)
       if (v[i] > -INFINITY) s += expf(v[i] - top);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    denom = s;
+    denom = lanes_sum<L>(s);
   }
   int my_id = -1;                                        // lane j keeps choice j
   float my_x = -INFINITY;
   for (int j = 0; j < p.k; ++j) {
     unsigned best = 0u;
-#pragma unroll
-    for (int i = 0; i < NE; ++i) best = max(best, key[i]);
-    const unsigned all = __reduce_max_sync(0xffffffffu, best);
-    if (all == 0u) break;                                // nobody is left
-    unsigned at = 0xffffffffu;
-#pragma unroll
-    for (int i = NE - 1; i >= 0; --i)
-      if (key[i] == all) at = unsigned(i * 32 + lane);
-    const int e = int(__reduce_min_sync(0xffffffffu, at));
-    float x = 0.f;
+    int at = 0x7fffffff;
 #pragma unroll
     for (int i = 0; i < NE; ++i)
-      if (i * 32 + lane == e) {
-        x = v[i];
+      if (key[i] > best) {                               // the lane's lowest index among equals
+        best = key[i];
+        at = i * L + sub;
+      }
+    if constexpr (L == 32) {
+      const unsigned all = __reduce_max_sync(0xffffffffu, best);
+      at = int(__reduce_min_sync(0xffffffffu, best == all ? unsigned(at) : 0x7fffffffu));
+      if (all == 0u) break;                              // nobody is left
+    } else {
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) {
+        const unsigned ob = __shfl_xor_sync(0xffffffffu, best, o);
+        const int oa = __shfl_xor_sync(0xffffffffu, at, o);
+        if (ob > best || (ob == best && oa < at)) {
+          best = ob;
+          at = oa;
+        }
+      }
+    }
+    float xv = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NE; ++i)
+      if (i * L + sub == at) {
+        xv = v[i];
         key[i] = 0u;
       }
-    x = __shfl_sync(0xffffffffu, x, e & 31);
-    if (lane == j) {
-      my_id = e;
-      my_x = x;
+    xv = __shfl_sync(0xffffffffu, xv, (lane & ~(L - 1)) | (at & (L - 1)));
+    if (sub == j && at != 0x7fffffff) {
+      my_id = at;
+      my_x = xv;
     }
   }
   float my_w;
   if (p.renorm) {
     // relative to the chosen ones' largest, so that they never all vanish; a sigmoid below e^-20 is an exponential
-    float m = my_x;                                      // lanes of no choice hold -inf; choices sit in the first eight
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float m = lanes_max<8>(my_x);                  // lanes of no choice hold -inf; choices sit in the first eight
     my_w = p.sigmoid && m > -20.f ? 1.f / (1.f + expf(-my_x)) : expf(my_x - m);
     if (my_id < 0) my_w = 0.f;
-    float s = my_w;
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const float s = lanes_sum<8>(my_w);
     my_w = s > 0.f ? my_w / s : 0.f;
   } else {
     my_w = my_id < 0 ? 0.f : p.sigmoid ? 1.f / (1.f + expf(-my_x)) : expf(my_x - top) / denom;
   }
-  if (lane < p.k) {
-    const long long at = (long long)token * p.k + lane;
-    p.ids[at] = my_id;
-    p.weights[at] = my_w * p.scale;
+  if (live && sub < p.k) {
+    const long long to = (long long)token * p.k + sub;
+    p.ids[to] = my_id;
+    p.weights[to] = my_w * p.scale;
   }
 }
 
-template <int NE>
+template <int L, int NE>
 __device__ __forceinline__ void choose_block(const RouteParams& p, int t0, int t1) {
+  constexpr int kStep = kRouteWarps * (32 / L);          // tokens a round of the block
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int t = t0 + warp; t < t1; t += kRouteWarps) choose_token<NE>(p, t, lane);
+  const int mine = warp * (32 / L) + lane / L;
+  float bias[NE], x[NE], next[NE];
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    const int e = i * L + (lane & (L - 1));
+    bias[i] = p.bias != nullptr && e < p.E ? __ldg(p.bias + e) : 0.f;
+  }
+  load_logits<L, NE>(p, t0 + mine, t0 + mine < t1, next);
+  for (int r0 = t0; r0 < t1; r0 += kStep) {              // the same number of rounds for every lane
+    const int t = r0 + mine;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) x[i] = next[i];
+    load_logits<L, NE>(p, t + kStep, t + kStep < t1, next);
+    choose_token<L, NE>(p, t, t < t1, bias, x);
+  }
 }
 
 // counts of the block's pairs, into cnt[0 .. E)
@@ -204,12 +246,12 @@ __device__ __forceinline__ void scan_experts(const int* tot, int* off, int E) {
 }
 
 // kOne: the only block does everything.  Otherwise this launch chooses and counts.
-template <int NE, bool kOne>
+template <int L, int NE, bool kOne>
 __global__ void __launch_bounds__(kRouteThreads)
 route_choose_kernel(const RouteParams p) {
   extern __shared__ int sm[];
   const int t0 = min(p.T, int(blockIdx.x) * p.tokens_per_block), t1 = min(p.T, t0 + p.tokens_per_block);
-  choose_block<NE>(p, t0, t1);
+  choose_block<L, NE>(p, t0, t1);
   count_block(p, t0, t1, sm);
   if (!kOne) {
     for (int e = threadIdx.x; e < p.E; e += kRouteThreads) p.counts[(long long)blockIdx.x * p.E + e] = sm[e];
@@ -232,14 +274,22 @@ route_place_kernel(const RouteParams p) {
   const int t0 = min(p.T, int(blockIdx.x) * p.tokens_per_block), t1 = min(p.T, t0 + p.tokens_per_block);
   for (int e = threadIdx.x; e < p.E; e += kRouteThreads) tot[e] = base[e] = 0;
   __syncthreads();
-  // all counts, blocks x experts flattened; adding whole numbers, in any order
-  const int cells = int(gridDim.x) * p.E;
-  for (int i = threadIdx.x; i < cells; i += kRouteThreads) {
-    const int c = p.counts[i];
-    if (c == 0) continue;
-    const int b = i / p.E, e = i - b * p.E;
-    atomicAdd(tot + e, c);
-    if (b < int(blockIdx.x)) atomicAdd(base + e, c);
+  // all counts: a thread adds up one expert over every few blocks; whole numbers, in any order
+  int width = 32;
+  while (width < p.E) width *= 2;                        // divides kRouteThreads (E <= 512)
+  {
+    const int e = int(threadIdx.x) & (width - 1), step = kRouteThreads / width;
+    if (e < p.E) {
+      int all = 0, before = 0;
+#pragma unroll 8
+      for (int b = int(threadIdx.x) / width; b < int(gridDim.x); b += step) {
+        const int c = p.counts[(long long)b * p.E + e];
+        all += c;
+        if (b < int(blockIdx.x)) before += c;
+      }
+      if (all != 0) atomicAdd(tot + e, all);
+      if (before != 0) atomicAdd(base + e, before);
+    }
   }
   __syncthreads();
   if (threadIdx.x < 32) scan_experts(tot, off, p.E);
@@ -251,25 +301,27 @@ route_place_kernel(const RouteParams p) {
   place_block(p, t0, t1, base, run, off[p.E]);
 }
 
-// Tokens that one block still routes faster than two launches do.
-constexpr int kOneBlockTokens = 128;
+constexpr int kSmallExperts = 64;                          // eight lanes a token
 
-int route_blocks(int64_t T) {
-  if (T <= kOneBlockTokens) return 1;
-  const int64_t want = (T + kRouteWarps - 1) / kRouteWarps, most = 148;     // the counts are read by every block
+// One block for up to eight rounds of its warps, otherwise one a run of tokens, at most one an SM (their counts are read
+// by every block).
+int route_blocks(int64_t T, int E) {
+  const int step = kRouteWarps * (E <= kSmallExperts ? 4 : 1);
+  if (T <= 8 * step) return 1;
+  const int64_t want = (T + step - 1) / step, most = 148;
   return int(want < most ? want : most);
 }
 
-template <int NE>
+template <int L, int NE>
 int launch_route(RouteParams p, cudaStream_t st) {
-  const int blocks = route_blocks(p.T);
+  const int blocks = route_blocks(p.T, p.E);
   p.tokens_per_block = (p.T + blocks - 1) / blocks;
   const size_t one = sizeof(int) * size_t(p.E + p.E + 1 + kRouteWarps * p.E);
   if (blocks == 1) {
-    route_choose_kernel<NE, true><<<1, kRouteThreads, one, st>>>(p);
+    route_choose_kernel<L, NE, true><<<1, kRouteThreads, one, st>>>(p);
     return launch_status();
   }
-  route_choose_kernel<NE, false><<<blocks, kRouteThreads, sizeof(int) * p.E, st>>>(p);
+  route_choose_kernel<L, NE, false><<<blocks, kRouteThreads, sizeof(int) * p.E, st>>>(p);
   if (int e = launch_status()) return e;
   route_place_kernel<<<blocks, kRouteThreads, one + sizeof(int) * p.E, st>>>(p);
   return launch_status();
@@ -282,7 +334,7 @@ extern "C" {
 
 int64_t samb_route_scratch_bytes(int64_t T, int E) {
   if (T < 0 || E <= 0 || E > samb::kMaxExperts) return 0;
-  const int blocks = samb::route_blocks(T);
+  const int blocks = samb::route_blocks(T, E);
   return blocks == 1 ? 0 : int64_t(blocks) * E * int64_t(sizeof(int));
 }
 
@@ -299,7 +351,7 @@ int samb_route_topk(const float* logits, int64_t ld, const float* bias, int64_t 
                         reinterpret_cast<uintptr_t>(slots) | reinterpret_cast<uintptr_t>(rows) |
                         reinterpret_cast<uintptr_t>(offsets) | reinterpret_cast<uintptr_t>(scratch);
   if (mis & 3u) return SAMB_E_ALIGN;
-  if (route_blocks(T) > 1 && scratch == nullptr) return SAMB_E_BADARG;
+  if (route_blocks(T, E) > 1 && scratch == nullptr) return SAMB_E_BADARG;
   if (int e = check_device_arch()) return e;
   RouteParams p;
   p.logits = logits; p.bias = bias; p.ids = ids; p.weights = weights; p.slots = slots; p.rows = rows; p.offsets = offsets;
@@ -307,11 +359,12 @@ int samb_route_topk(const float* logits, int64_t ld, const float* bias, int64_t 
   p.ld = ld; p.T = int(T); p.E = E; p.k = k;
   p.sigmoid = sigmoid != 0; p.renorm = renorm != 0; p.scale = scale;
   auto st = static_cast<cudaStream_t>(stream);
-  if (E <= 32) return launch_route<1>(p, st);
-  if (E <= 64) return launch_route<2>(p, st);
-  if (E <= 128) return launch_route<4>(p, st);
-  if (E <= 256) return launch_route<8>(p, st);
-  return launch_route<16>(p, st);
+  if (E <= 16) return launch_route<8, 2>(p, st);
+  if (E <= 32) return launch_route<8, 4>(p, st);
+  if (E <= kSmallExperts) return launch_route<8, 8>(p, st);
+  if (E <= 128) return launch_route<32, 4>(p, st);
+  if (E <= 256) return launch_route<32, 8>(p, st);
+  return launch_route<32, 16>(p, st);
 }
 
 }  // extern "C"

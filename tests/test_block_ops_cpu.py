@@ -57,7 +57,7 @@ def test_rotary_refusals(lib, want, change):
     assert _rot(lib, **change) == want
 
 
-def _route(lib, x=P, ld=16, T=300, E=16, k=2, ids=P, w=P, slots=P, rows=P, off=P, scratch=P):
+def _route(lib, x=P, ld=16, T=3000, E=16, k=2, ids=P, w=P, slots=P, rows=P, off=P, scratch=P):
     return lib.samb_route_topk(x, ld, None, T, E, k, 0, 1, 1.0, ids, w, slots, rows, off, scratch, None)
 
 
