@@ -622,19 +622,19 @@ def _block_norm(fn: str, h, residual, post, pre, gate, res_scale, eps, rms, out,
         if gates == 0 or rows % gates:
             raise RuntimeError(f"gate: {gates} vectors do not divide {rows} rows")
     if out is None:
-        out, ldx = torch.empty((rows, C), dtype=dtype, device=h.device), C
+        out, ldx = torch.empty_like(h), C                 # rows of unit inner stride: a dense copy is row-major
     else:
         ldx = _like(out, dtype, dev, shape, "out")
     y = scale = None
     if quant:
-        y = torch.empty((rows, C), dtype=torch.int8, device=h.device)
-        scale = torch.empty((rows,), dtype=_F32, device=h.device)
+        y = torch.empty(rows, C, dtype=torch.int8, device=h.device)
+        scale = torch.empty(rows, dtype=_F32, device=h.device)
         _lib.check(_lib.load().samb_block_norm_quant_i8(
             h.data_ptr(), ldh, pr, ldr, pgg, pgb, pqg, pqb, pg, gates, res_scale, eps, rms, out.data_ptr(), ldx,
             y.data_ptr(), scale.data_ptr(), rows, C, _stream()), fn)
     else:
         if pre is not None:
-            y = torch.empty((rows, C), dtype=dtype, device=h.device)
+            y = torch.empty_like(h)
             py = y.data_ptr()
         _lib.check(_lib.load().samb_block_norm(
             h.data_ptr(), ldh, pr, ldr, pgg, pgb, pqg, pqb, pg, gates, res_scale, eps, dtype is _F16, rms,
@@ -719,7 +719,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, interl
     if freqs.dim() != 1 or not freqs.is_contiguous():
         raise RuntimeError("freqs: expected a contiguous 1-D tensor")
     if out is None:
-        out = torch.empty((planes, rows, d), dtype=dtype, device=x.device)
+        out = torch.empty(planes, rows, d, dtype=dtype, device=x.device)
         ops_, ors, oes = rows * d, d, 1
     else:
         _here(out, dtype, dev, "out")
@@ -766,8 +766,8 @@ def route_topk(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] = None
     n = T * k
     scratch = lib.samb_route_scratch_bytes(T, E) // 4
     # one allocation for the whole numbers: ids, slots, rows, offsets, scratch
-    buf = torch.empty((3 * n + E + 1 + scratch,), dtype=_I32, device=logits.device)
-    weights = torch.empty((T, k), dtype=_F32, device=logits.device)
+    buf = torch.empty(3 * n + E + 1 + scratch, dtype=_I32, device=logits.device)
+    weights = torch.empty(T, k, dtype=_F32, device=logits.device)
     at = buf.data_ptr()
     _lib.check(lib.samb_route_topk(
         logits.data_ptr(), ld, _vector(bias, "bias", dev, (E,)) if bias is not None else None, T, E, k, sigmoid, renorm,
@@ -799,14 +799,14 @@ def _grouped(kind, a, a_scale, w, w_scale, offsets, rows, bias, gelu, out, dtype
         prow = _indexes(rows, "rows", dev, S)
         room = lib.samb_gemm_grouped_scratch_bytes(S, E, K, int8)
         if room:                                          # room to put the rows of a large product in order
-            scratch = torch.empty((room,), dtype=torch.uint8, device=a.device)
+            scratch = torch.empty(room, dtype=torch.uint8, device=a.device)
             psc = scratch.data_ptr()
     if bias is not None:
         pbias = _vector(bias, "bias", dev, (E, N))
         epi |= EPI_BIAS
     poff = _indexes(offsets, "offsets", dev, E + 1)
     if out is None:
-        out, ldo = torch.empty((S, N), dtype=odt, device=a.device), N
+        out, ldo = torch.empty(S, N, dtype=odt, device=a.device), N
     else:
         ldo = _like(out, odt, dev, (S, N), "out")
     if N <= 1:
@@ -866,7 +866,7 @@ def combine_topk(x: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, re
         ldr = _like(residual, dtype, dev, (T, C), "residual")
         pr = residual.data_ptr()
     if out is None:
-        out, ldo = torch.empty((T, C), dtype=dtype, device=x.device), C
+        out, ldo = torch.empty(T, C, dtype=dtype, device=x.device), C
     else:
         ldo = _like(out, dtype, dev, (T, C), "out")
     _lib.check(_lib.load().samb_combine_topk(
