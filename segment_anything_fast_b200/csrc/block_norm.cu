@@ -13,6 +13,8 @@
 //   M2 = sum_w M2_w + n_w (mean_w - mean)^2,
 // so a norm costs one block barrier for four rows and no difference of large squares is ever taken.  The four rows'
 // sums share their shuffles: halves of the warp trade rows first, 6 shuffles instead of 20.
+// Bound by HBM: 235 us for 131072 x 1280 bf16 with both norms and a gate an image (1.34 GB, 5.7 TB/s); a row at a time through
+// registers took 635 us, held up by its barriers and shuffles.
 #include "elem16.cuh"
 
 namespace samb {
@@ -54,64 +56,49 @@ __device__ __forceinline__ void fill8(float (&v)[8], float x) {
   for (int j = 0; j < 8; ++j) v[j] = x;
 }
 
-// Statistics of kRows rows whose columns are spread over the block: on return sub[i] is what to subtract and
-// mul[i] what to multiply by.  `stat` is shared scratch for kRows * warps pairs; a caller alternates between two of
-// them, so that a buffer's next writes are a barrier away from its last reads.
-template <bool kRms, int kRows>
-__device__ __forceinline__ void row_stats(const float (&v)[kRows][8], bool live, int C, float eps, float2* stat,
-                                          float (&sub)[kRows], float (&mul)[kRows]) {
+// Statistics of a row whose columns are spread over the block: on return sub is what to subtract and mul what to
+// multiply by.  `stat` is shared scratch for a pair a warp; a caller alternates between two of them, so that a buffer's
+// next writes are a barrier away from its last reads.
+template <bool kRms>
+__device__ __forceinline__ void row_stats(const float (&v)[8], bool live, int C, float eps, float2* stat, float& sub,
+                                          float& mul) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const float inv_n = 1.0f / float(min(256, C - warp * 256));      // columns of this warp
-  float2 mine[kRows];
-#pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    float mean = 0.f, m2 = 0.f;
-    if (!kRms) {
-      float s = 0.f;
-      if (live) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s += v[i][j];
-      }
-      mean = warp_sum(s) * inv_n;
-    }
+  float mean = 0.f, m2 = 0.f;
+  if (!kRms) {
+    float s = 0.f;
     if (live) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float d = v[i][j] - mean;
-        m2 = fmaf(d, d, m2);
-      }
+      for (int j = 0; j < 8; ++j) s += v[j];
     }
-    mine[i] = make_float2(mean, warp_sum(m2));
+    mean = warp_sum(s) * (1.0f / float(min(256, C - warp * 256)));      // over the columns of this warp
   }
-  if (warps > 1) {
-    if (lane == 0) {
+  if (live) {
 #pragma unroll
-      for (int i = 0; i < kRows; ++i) stat[warp * kRows + i] = mine[i];
+    for (int j = 0; j < 8; ++j) {
+      const float d = v[j] - mean;
+      m2 = fmaf(d, d, m2);
     }
-    __syncthreads();
   }
+  m2 = warp_sum(m2);
   const float inv_c = 1.0f / float(C);
-#pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    float mean = mine[i].x, m2 = mine[i].y;
-    if (warps > 1) {
-      mean = 0.f;
-      if (!kRms) {                                       // around the first warp's: a constant row stays exact
-        const float first = stat[i].x;
-        for (int w = 1; w < warps; ++w) mean = fmaf(stat[w * kRows + i].x - first, float(min(256, C - w * 256)), mean);
-        mean = fmaf(mean, inv_c, first);
-      }
-      m2 = 0.f;
-      for (int w = 0; w < warps; ++w) {
-        const float2 s = stat[w * kRows + i];
-        const float d = s.x - mean;
-        m2 += s.y;
-        if (!kRms) m2 = fmaf(d * d, float(min(256, C - w * 256)), m2);
-      }
+  if (warps > 1) {
+    if (lane == 0) stat[warp] = make_float2(mean, m2);
+    __syncthreads();
+    mean = m2 = 0.f;
+    if (!kRms) {                                         // around the first warp's: a constant row stays exact
+      const float first = stat[0].x;
+      for (int w = 1; w < warps; ++w) mean = fmaf(stat[w].x - first, float(min(256, C - w * 256)), mean);
+      mean = fmaf(mean, inv_c, first);
     }
-    sub[i] = mean;
-    mul[i] = rsqrtf(fmaf(m2, inv_c, eps));
+    for (int w = 0; w < warps; ++w) {
+      const float2 s = stat[w];
+      const float d = s.x - mean;
+      m2 += s.y;
+      if (!kRms) m2 = fmaf(d * d, float(min(256, C - w * 256)), m2);
+    }
   }
+  sub = mean;
+  mul = rsqrtf(fmaf(m2, inv_c, eps));
 }
 
 // The sum over the warp of four values: afterwards the lanes of group l >> 3 all hold the sum of value l >> 3.
@@ -326,13 +313,12 @@ block_norm_rows_kernel(const NormParams p) {
 
 // One row at a time: few rows, where latency counts, and wide ones.  kWide: up to 32 warps a block (C up to 8192), which
 // leaves 64 registers a thread: the parameters are then read where they are used.
-template <typename T, bool kRms, bool kQuant, int kRows, bool kWide>
+template <typename T, bool kRms, bool kQuant, bool kWide>
 __global__ void __launch_bounds__(kWide ? 1024 : 256)
 block_norm_kernel(const NormParams p) {
-  constexpr int kPairs = kRows * (kWide ? 32 : 8);
-  __shared__ float2 s_post[2][kPairs], s_pre[2][kPairs];
-  __shared__ float s_max[kPairs];            // used between the barriers of two norms
-  int turn = 0;
+  constexpr int kMaxWarps = kWide ? 32 : 8;
+  __shared__ float2 s_post[2][kMaxWarps], s_pre[2][kMaxWarps];
+  __shared__ float s_max[kMaxWarps];         // used between the barriers of two norms
   const int c = int(threadIdx.x) * 8;
   const bool live = c < p.C;
   const int begin = int(blockIdx.x) * p.rows_per_block;
@@ -340,7 +326,6 @@ block_norm_kernel(const NormParams p) {
   const bool has_post = p.post_g != nullptr, has_pre = p.pre_g != nullptr;
 
   float pg[8], pb[8], qg[8], qb[8];          // post's gain and offset (times the gate), pre's gain and offset
-  fill8(pg, 1.f); fill8(pb, 0.f); fill8(qg, 1.f); fill8(qb, 0.f);
   auto load_post = [&](int row) {
     fill8(pg, 1.f);
     fill8(pb, 0.f);
@@ -358,83 +343,54 @@ block_norm_kernel(const NormParams p) {
     }
   };
   auto load_pre = [&]() {
+    fill8(qg, 1.f);
+    fill8(qb, 0.f);
     if (!live) return;
     if (has_pre) load8(p.pre_g, c, qg);
     if (p.pre_b != nullptr) load8(p.pre_b, c, qb);
   };
-  int next_gate = begin;                     // first row that needs another gate vector than the one held
+  int next_gate = begin, turn = 0;           // next_gate: first row that needs another gate vector than the one held
   if (!kWide) load_pre();
 
-  for (int row0 = begin; row0 < end; row0 += kRows, turn ^= 1) {
-    uint4 hr[kRows], rr[kRows];
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      hr[i] = rr[i] = make_uint4(0u, 0u, 0u, 0u);
-      const int row = row0 + i;
-      if (live && row < end) {
-        hr[i] = *(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.h) + row * p.ldh + c));
-        if (p.r != nullptr) rr[i] = *(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.r) + row * p.ldr + c));
-      }
+  for (int row = begin; row < end; ++row, turn ^= 1) {
+    uint4 hr = make_uint4(0u, 0u, 0u, 0u), rr = hr;
+    if (live) {
+      hr = *(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.h) + row * p.ldh + c));
+      if (p.r != nullptr) rr = *(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.r) + row * p.ldr + c));
     }
-    float v[kRows][8], sub[kRows], mul[kRows];
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) T::unpack(hr[i], v[i]);
-    if (has_post) {
-      row_stats<kRms, kRows>(v, live, p.C, p.eps, s_post[turn], sub, mul);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kRows; ++i) { sub[i] = 0.f; mul[i] = 1.f; }
+    if (kWide || row >= next_gate) {         // the same for every thread
+      load_post(row);
+      next_gate = (row / p.rows_per_gate + 1) * p.rows_per_gate;     // <= rows: whole blocks of rows
     }
+    float v[8], r[8], sub = 0.f, mul = 1.f;
+    T::unpack(hr, v);
+    T::unpack(rr, r);
+    if (has_post) row_stats<kRms>(v, live, p.C, p.eps, s_post[turn], sub, mul);
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      const int row = row0 + i;
-      if (row < end && (kWide || row >= next_gate)) {                // the same for every thread
-        load_post(row);
-        next_gate = (row / p.rows_per_gate + 1) * p.rows_per_gate;   // <= rows: whole blocks of rows
-      }
-      float r[8];
-      T::unpack(rr[i], r);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = fmaf((v[i][j] - sub[i]) * mul[i], pg[j], fmaf(p.res_scale, r[j], pb[j]));
-      if (live && row < end)
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.x) + row * p.ldx + c) = T::pack(v[i]);
-    }
+    for (int j = 0; j < 8; ++j) v[j] = fmaf((v[j] - sub) * mul, pg[j], fmaf(p.res_scale, r[j], pb[j]));
+    if (live) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.x) + row * p.ldx + c) = T::pack(v);
     if (!has_pre) continue;
-    row_stats<kRms, kRows>(v, live, p.C, p.eps, s_pre[turn], sub, mul);
+    row_stats<kRms>(v, live, p.C, p.eps, s_pre[turn], sub, mul);
     if (kWide) load_pre();
-    uint4 out[kRows];
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      float f[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = fmaf((v[i][j] - sub[i]) * mul[i], qg[j], qb[j]);
-      out[i] = T::pack(f);
-      if (!kQuant && live && row0 + i < end)
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.y) + (long long)(row0 + i) * p.C + c) = out[i];
+    for (int j = 0; j < 8; ++j) v[j] = fmaf((v[j] - sub) * mul, qg[j], qb[j]);
+    const uint4 out = T::pack(v);
+    if (!kQuant) {
+      if (live) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.y) + (long long)row * p.C + c) = out;
+      continue;
     }
-    if (kQuant) {
-      // the rounded row, as a quantised Linear fed with 16-bit rows would see it
-      const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-      float amax[kRows];
-#pragma unroll
-      for (int i = 0; i < kRows; ++i) {
-        const float m = live ? absmax_fold(absmax8(__floats2bfloat162_rn(0.f, 0.f), out[i])) : 0.f;
-        amax[i] = warp_max(m);
-        if (warps > 1 && lane == 0) s_max[warp * kRows + i] = amax[i];
-      }
-      if (warps > 1) __syncthreads();
-#pragma unroll
-      for (int i = 0; i < kRows; ++i) {
-        for (int w = 0; warps > 1 && w < warps; ++w) amax[i] = fmaxf(amax[i], s_max[w * kRows + i]);
-        float sc, inv_sc;
-        row_scale(amax[i], sc, inv_sc);
-        if (row0 + i < end) {
-          if (threadIdx.x == 0) p.y_scale[row0 + i] = sc;
-          if (live)
-            *reinterpret_cast<uint2*>(static_cast<int8_t*>(p.y) + (long long)(row0 + i) * p.C + c) = quant8(out[i], sc, inv_sc);
-        }
-      }
+    // the rounded row, as a quantised Linear fed with 16-bit rows would see it
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    float amax = warp_max(live ? absmax_fold(absmax8(__floats2bfloat162_rn(0.f, 0.f), out)) : 0.f);
+    if (warps > 1) {
+      if (lane == 0) s_max[warp] = amax;
+      __syncthreads();
+      for (int w = 0; w < warps; ++w) amax = fmaxf(amax, s_max[w]);
     }
+    float sc, inv_sc;
+    row_scale(amax, sc, inv_sc);
+    if (threadIdx.x == 0) p.y_scale[row] = sc;
+    if (live) *reinterpret_cast<uint2*>(static_cast<int8_t*>(p.y) + (long long)row * p.C + c) = quant8(out, sc, inv_sc);
   }
 }
 
@@ -467,8 +423,8 @@ int launch_typed(NormParams& p, cudaStream_t st) {
   const long long most = (long long)sm_count() * (wide ? 2 : 8);
   p.rows_per_block = int((p.rows + most - 1) / most);
   const unsigned blocks = unsigned((p.rows + p.rows_per_block - 1) / p.rows_per_block);
-  if (wide) block_norm_kernel<T, kRms, kQuant, 1, true><<<blocks, threads, 0, st>>>(p);
-  else block_norm_kernel<T, kRms, kQuant, 1, false><<<blocks, threads, 0, st>>>(p);
+  if (wide) block_norm_kernel<T, kRms, kQuant, true><<<blocks, threads, 0, st>>>(p);
+  else block_norm_kernel<T, kRms, kQuant, false><<<blocks, threads, 0, st>>>(p);
   return launch_status();
 }
 
@@ -484,13 +440,13 @@ int launch_block_norm(const void* h, int64_t ldh, const void* r, int64_t ldr, co
       (y != nullptr && ((y == h && (quant || ldh != C)) || (y == r && (quant || ldr != C)))))
     return SAMB_E_BADARG;
   if (gate != nullptr && (gate_rows <= 0 || rows % gate_rows)) return SAMB_E_SHAPE;
-  if (C % 8 || C > 8192 || rows >= (int64_t(1) << 31)) return SAMB_E_SHAPE;
+  if (C % 8 || C > 8192 || rows > 0x7fffff00) return SAMB_E_SHAPE;          // row numbers stay in 32 bits
   if (ldh % 8 || ldx % 8 || ldh < C || ldx < C || (r != nullptr && (ldr % 8 || ldr < C))) return SAMB_E_SHAPE;
   const uintptr_t mis = reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(r) | reinterpret_cast<uintptr_t>(x) |
                         reinterpret_cast<uintptr_t>(post_g) | reinterpret_cast<uintptr_t>(post_b) |
                         reinterpret_cast<uintptr_t>(pre_g) | reinterpret_cast<uintptr_t>(pre_b) |
                         reinterpret_cast<uintptr_t>(gate) | reinterpret_cast<uintptr_t>(y);
-  if (mis & 15u) return SAMB_E_ALIGN;
+  if ((mis & 15u) || (reinterpret_cast<uintptr_t>(y_scale) & 3u)) return SAMB_E_ALIGN;
   if (int e = check_device_arch()) return e;
   if (rows == 0) return SAMB_OK;
   NormParams p;

@@ -4,7 +4,7 @@
 // CTA works the tile list out for itself: the prefix over the experts of their row tiles, times the column tiles.
 //
 // Three kernels.  On CTA pairs (256 x 256 tiles, cta_group::2, each CTA loads its 128 rows of A and half of W) for groups
-// of a few hundred rows and more; on single CTAs (128 x 256, 128 or 64) below, where the weights' bytes count and the
+// of some 500 rows and more; on single CTAs (128 rows, 64 to 256 columns) below, where the weights' bytes count and the
 // number of tiles is what spreads their stream over the SMs; and for a handful of rows in all (serving a token or two) dot
 // products by warps, which have neither tensor maps to build nor a pipeline to fill.
 //
@@ -12,7 +12,12 @@
 // `rows` the single-CTA kernel has a warp per stage fetch them with 16-byte cp.async into the same swizzled places.  The
 // pair kernel would gather every row again for each of its column tiles, faster than cp.async delivers them (774 us
 // against 590 us for rows in order at 65536 x 5120 x 1280; TMA's own gather of four rows, at some 85 cycles an
-// instruction, took 2110 us), so its rows are put in order first, in caller scratch: a pass at copy bandwidth (30 us).
+// instruction, took 2110 us), so large products have their rows put in order first, in caller scratch: a pass at copy
+// bandwidth (40 us there).
+//
+// Measured, one B200: 65536 x 5120 x 1280 bf16 with 16 experts, gathered, bias and GELU: 650 us = 1.32 PFLOP/s (one dense
+// product of that size: 578 us here, 587 us by the vendor library); 16384 x 5120 x 1280 int8: 111 us = 1.9 POP/s; 2062 x 1280 x
+// 5120 f16: 48 us, 4.9 TB/s; one token with two experts of 5120 x 1280: 8.8 us, 3.0 TB/s.
 //
 // A tile computes all its rows whatever its expert has left (the rows behind them in shared memory may be anything: a
 // row of the product depends on its own row of A alone), but stores only its own: whole tiles leave by TMA, the last
@@ -120,13 +125,13 @@ struct TileWalk {
 };
 
 // A gathering warp owns one stage of the ring: for every STAGES-th slab it waits until the stage is free, fetches 128
-// rows of A (from row `skip` of the tile) with 32 cp.async a lane, eight lanes a row, waits for them and passes the slab
-// on.  Rows whose index lies outside A and columns behind K are filled with zeros.  cp.async writes through the generic proxy and the
-// tensor core reads through the async one; the fence between the two waits for the thread's copies in flight, so a
-// thread with several slabs in flight would pay the whole memory latency for each of them.  Here the warps overlap.
+// rows of A with 32 cp.async a lane, eight lanes a row, waits for them and passes the slab on.  Rows whose index lies
+// outside A and columns behind K are filled with zeros.  cp.async writes through the generic proxy and the tensor core
+// reads through the async one; the fence between the two waits for the thread's copies in flight, so a thread with
+// several slabs in flight would pay the whole memory latency for each of them.  Here the warps overlap.
 template <int STAGES, int kStageBytes, typename Arrive>
 __device__ __forceinline__ void gather_role(const GroupedParams& p, TileWalk w, uint8_t* smem, uint64_t* empty_bar,
-                                            volatile int* abort_flag, int stage, int skip, int tile0, int step, int num_tiles,
+                                            volatile int* abort_flag, int stage, int tile0, int step, int num_tiles,
                                             Arrive arrive) {
   const int lane = threadIdx.x & 31;
   const int unit = lane & 7, quarter = lane >> 3;
@@ -141,7 +146,7 @@ __device__ __forceinline__ void gather_role(const GroupedParams& p, TileWalk w, 
     int idx[4];                                          // rows 32 i + lane of the tile
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int m = skip + i * 32 + lane;
+      const int m = i * 32 + lane;
       const int r = m < w.rows ? __ldg(p.rows + w.m0 + m) : -1;
       idx[i] = r < p.a_rows ? r : -1;
     }
@@ -152,7 +157,7 @@ __device__ __forceinline__ void gather_role(const GroupedParams& p, TileWalk w, 
       const uint8_t* base = p.a + (inside ? k0 : 0);
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
-        if (j * 4 >= w.rows - skip) break;               // what lies behind the tile's rows may be anything
+        if (j * 4 >= w.rows) break;                     // what lies behind the tile's rows may be anything
         const int r = __shfl_sync(0xffffffffu, idx[j >> 3], (j & 7) * 4 + quarter);
         const bool there = inside && r >= 0;
         const uint8_t* s = base + (there ? r : 0) * p.a_pitch;
@@ -336,7 +341,7 @@ grouped_one_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     }
   } else if (kGather && warp >= ONE_THREADS / 32) {
     // ------------------------------------------------------------------ gathering warps
-    gather_role<STAGES, STAGE_BYTES>(p, w, smem, empty_bar, abort_flag, warp - ONE_THREADS / 32, 0, int(blockIdx.x),
+    gather_role<STAGES, STAGE_BYTES>(p, w, smem, empty_bar, abort_flag, warp - ONE_THREADS / 32, int(blockIdx.x),
                                      int(gridDim.x), num_tiles, [&](int s) { mbar_arrive(&full_bar[s]); });
   } else {
     // ------------------------------------------------------------------ epilogue
@@ -844,18 +849,18 @@ void launch_few(const uint8_t* W, long long w_pitch, long long w_stride, const G
   else grouped_few_kernel<kType, 1><<<grid, 32 * FEW_WARPS, 0, st>>>(W, w_pitch, w_stride, p, gelu);
 }
 
-#ifndef SAMB_FEW_SLOTS
-#define SAMB_FEW_SLOTS 8
-#endif
-constexpr int64_t kFewSlots = SAMB_FEW_SLOTS;
+// Rows in all up to which the dot products win.  16 experts, us, against the tile kernel: 5120 x 1280 bf16 15 / 19 at 8 rows,
+// 35 / 45 at 12, 34 / 43 at 16, 53 / 36 at 24; 1280 x 5120: 18 / 57 at 8, 38 / 59 at 12, 59 / 33 at 16; int8 5120 x 1280: 11 / 12 at 8,
+// 12 / 21 at 12, 18 / 19 at 16.
+constexpr int64_t kFewSlots = 8;
 
 // Rows of A in the order of the slots, packed: 16-byte vectors, several loads a thread in flight.  A row that does not
-// exist is zeros; slots behind the last expert's are left out.
+// exist is zeros.
 constexpr int kOrderVecs = 4;
 __global__ void __launch_bounds__(256)
 order_rows_kernel(const GroupedParams p, uint4* __restrict__ to) {
   const unsigned nv = unsigned(p.k_bytes >> 4);
-  const long long last = (long long)min(max(__ldg(p.offsets + p.E), 0), int(p.S)) * nv;
+  const long long last = p.S * nv;
   const long long i0 = (long long)blockIdx.x * (256 * kOrderVecs) + threadIdx.x;
   uint4 v[kOrderVecs];
 #pragma unroll
@@ -950,6 +955,7 @@ int launch_grouped(int type, const void* A, int64_t lda, int64_t a_rows, const f
   if (((epilogue & SAMB_EPI_BIAS) != 0) != (bias != nullptr)) return SAMB_E_BADARG;
   if (S > 0 && (A == nullptr || W == nullptr || out == nullptr || offsets == nullptr || a_rows == 0)) return SAMB_E_BADARG;
   if (type == kTypeI8 && S > 0 && (a_scale == nullptr || w_scale == nullptr)) return SAMB_E_BADARG;
+  if (out != nullptr && (out == A || out == W)) return SAMB_E_BADARG;
   const int esz = type == kTypeI8 ? 1 : 2, kmul = 16 / esz;
   if (E > kMaxExperts || N % 8 || K % kmul || lda % kmul || ldw % kmul || w_stride % kmul || ldo % 8) return SAMB_E_SHAPE;
   if (lda < K || ldw < K || ldo < N || (E > 1 && w_stride < ldw * (N - 1) + K)) return SAMB_E_SHAPE;

@@ -596,6 +596,16 @@ def _like(t: torch.Tensor, dtype: torch.dtype, dev: int, shape, name: str) -> in
     return _matrix(t, name)
 
 
+def _status(t: torch.Tensor, dev: int) -> int:
+    """Pointer of the device's status word.  It outlives the call, so a capture must not be what allocates it."""
+    w = _status_words.get(dev)
+    if w is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("make one call on this device before capturing it into a graph")
+        w = status_word(t.device)
+    return w.data_ptr()
+
+
 def _block_norm(fn: str, h, residual, post, pre, gate, res_scale, eps, rms, out, quant):
     dtype, dev = _half(h, "h")
     ldh = _matrix(h, "h")
@@ -813,7 +823,7 @@ def _grouped(kind, a, a_scale, w, w_scale, offsets, rows, bias, gelu, out, dtype
         ldw = K
     if E <= 1:
         ws = 0
-    st = status_word(a.device).data_ptr()
+    st = _status(a, dev)
     if int8:
         _lib.check(lib.samb_gemm_i8_grouped(
             a.data_ptr(), lda, M, _vector(a_scale, "a_scale", dev, (M,)), prow, w.data_ptr(), ldw, ws,

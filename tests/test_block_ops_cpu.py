@@ -25,7 +25,7 @@ def _norm(lib, h=P, ldh=64, r=2 * P, ldr=64, pg=P, pb=P, qg=P, qb=P, gate=None, 
     (BAD, dict(h=None)), (BAD, dict(x=None)), (BAD, dict(rows=-1)), (BAD, dict(C=0)), (BAD, dict(pg=None)),
     (BAD, dict(qg=None)), (BAD, dict(y=None)), (BAD, dict(y=3 * P)), (BAD, dict(x=P, ldx=72)), (BAD, dict(x=2 * P, ldx=72)),
     (BAD, dict(y=P, ldh=72)), (BAD, dict(y=2 * P, ldr=72)),
-    (SHAPE, dict(C=60)), (SHAPE, dict(C=8200, ldh=8200, ldr=8200, ldx=8200)), (SHAPE, dict(rows=1 << 31)),
+    (SHAPE, dict(C=60)), (SHAPE, dict(C=8200, ldh=8200, ldr=8200, ldx=8200)), (SHAPE, dict(rows=(1 << 31) - 4)),
     (SHAPE, dict(ldh=56)), (SHAPE, dict(ldh=68)), (SHAPE, dict(ldr=60)), (SHAPE, dict(ldx=63)),
     (SHAPE, dict(gate=P, gates=4)), (SHAPE, dict(gate=P, gates=0)),
     (ALIGN, dict(h=P + 2)), (ALIGN, dict(gate=P + 4, gates=2)), (ALIGN, dict(y=5 * P + 8)), (ALIGN, dict(pg=P + 4))])
@@ -38,6 +38,7 @@ def test_block_norm_quant_refusals(lib):
     assert f(P, 64, None, 0, None, None, P, None, None, 0, 1.0, 1e-6, 0, 2 * P, 64, 3 * P, None, 6, 64, None) == BAD
     assert f(P, 64, None, 0, None, None, None, None, None, 0, 1.0, 1e-6, 0, 2 * P, 64, None, P, 6, 64, None) == BAD
     assert f(P, 64, None, 0, None, None, P, None, None, 0, 1.0, 1e-6, 0, 2 * P, 64, P, 4 * P, 6, 64, None) == BAD   # yq over h
+    assert f(P, 64, None, 0, None, None, P, None, None, 0, 1.0, 1e-6, 0, 2 * P, 64, 3 * P, 4 * P + 2, 6, 64, None) == ALIGN
 
 
 def _rot(lib, x=P, ps=640, rs=64, pos=P, p64=0, period=5, axes=1, freqs=P, rot=64, out=2 * P, ops=640, ors=64, planes=3, rows=10,
@@ -64,12 +65,12 @@ def _route(lib, x=P, ld=16, T=3000, E=16, k=2, ids=P, w=P, slots=P, rows=P, off=
 @pytest.mark.parametrize("want,change", [
     (BAD, dict(x=None)), (BAD, dict(off=None)), (BAD, dict(slots=None)), (BAD, dict(T=-1)), (BAD, dict(k=0)),
     (BAD, dict(scratch=None)), (SHAPE, dict(k=9)), (SHAPE, dict(E=513, ld=513)), (SHAPE, dict(ld=15)),
-    (SHAPE, dict(E=1, k=2)), (SHAPE, dict(T=1 << 30)), (ALIGN, dict(ids=P + 2))])
+    (SHAPE, dict(E=1, k=2)), (SHAPE, dict(T=1 << 30)), (SHAPE, dict(T=(1 << 31) - 1, k=1)), (ALIGN, dict(ids=P + 2))])
 def test_route_refusals(lib, want, change):
     assert _route(lib, **change) == want
 
 
-def _grouped(lib, a=P, lda=64, m=100, rows=P, w=P, ldw=64, ws=64 * 32, bias=P, off=P, out=P, ldo=32, S=200, E=4, N=32, K=64,
+def _grouped(lib, a=P, lda=64, m=100, rows=P, w=2 * P, ldw=64, ws=64 * 32, bias=P, off=P, out=3 * P, ldo=32, S=200, E=4, N=32, K=64,
              epi=1, st=P, scr=None):
     return lib.samb_gemm_grouped(a, lda, m, rows, w, ldw, ws, bias, off, out, ldo, S, E, N, K, 0, epi, scr, st, None)
 
@@ -77,7 +78,7 @@ def _grouped(lib, a=P, lda=64, m=100, rows=P, w=P, ldw=64, ws=64 * 32, bias=P, o
 @pytest.mark.parametrize("want,change", [
     (BAD, dict(a=None)), (BAD, dict(w=None)), (BAD, dict(off=None)), (BAD, dict(out=None)), (BAD, dict(st=None)),
     (BAD, dict(bias=None)), (BAD, dict(epi=0)), (BAD, dict(epi=4 + 1)), (BAD, dict(epi=8)), (BAD, dict(S=-1)),
-    (BAD, dict(m=0)), (BAD, dict(E=0)),
+    (BAD, dict(m=0)), (BAD, dict(E=0)), (BAD, dict(out=P)), (BAD, dict(out=2 * P)),
     (SHAPE, dict(N=36, ldo=40)), (SHAPE, dict(K=60)), (SHAPE, dict(lda=56)), (SHAPE, dict(ldw=60)), (SHAPE, dict(ldo=24)),
     (SHAPE, dict(ws=64 * 16)), (SHAPE, dict(rows=None)), (SHAPE, dict(E=513)), (SHAPE, dict(S=(1 << 31) - 1)),
     (SHAPE, dict(S=(1 << 31) - 200, N=1 << 20, ldo=1 << 20, ws=1 << 26)),
@@ -88,7 +89,7 @@ def test_grouped_refusals(lib, want, change):
 
 def test_grouped_i8_refusals(lib):
     def call(scale=P, ws=P, K=64):
-        return lib.samb_gemm_i8_grouped(P, 64, 100, scale, P, P, 64, 64 * 32, ws, None, P, P, 32, 200, 4, 32, K, 0, None, P, None)
+        return lib.samb_gemm_i8_grouped(P, 64, 100, scale, P, 2 * P, 64, 64 * 32, ws, None, P, 3 * P, 32, 200, 4, 32, K, 0, None, P, None)
     assert call(scale=None) == BAD and call(ws=None) == BAD
     assert call(K=56) == SHAPE                       # 8-element steps are enough for 16-bit types only
 

@@ -407,11 +407,12 @@ def test_gemm_grouped(ops, counts, behind, N, K, pad, gather, t):
 
 
 @pytest.mark.parametrize("t", [BF16, torch.int8])
-@pytest.mark.parametrize("S", [6, 200])
-def test_gemm_grouped_bad_indexes(ops, S, t):
-    """Indexes outside A are rows of zeros; offsets outside the buffer or falling back reach nothing outside."""
+@pytest.mark.parametrize("S,K", [(6, 64), (200, 64), (200, 1024), (2400, 1024)])
+def test_gemm_grouped_bad_indexes(ops, S, K, t):
+    """Indexes outside A are rows of zeros; offsets outside the buffer or falling back reach nothing outside.  (Warp dot
+    products, rows gathered in the kernel, put in order first, and on CTA pairs.)"""
     g = gen(S)
-    a, w, sa, sw = operands(g, t, 50, 4, 136, 64)
+    a, w, sa, sw = operands(g, t, 50, 4, 136, K)
     rows = torch.randint(0, 50, (S,), generator=g, device="cuda", dtype=torch.int32)
     rows[1], rows[3], rows[4] = -1, 50, 2 ** 31 - 1
     bias = rand(g, 4, 136)
@@ -543,6 +544,79 @@ def test_wrapper_refusals(ops):
         with pytest.raises(RuntimeError):
             call()
             pytest.fail(f"call {n} was not refused")
+
+
+def test_tensors_of_another_device_are_refused(ops, monkeypatch):
+    h, f = torch.zeros(8, 64, dtype=BF16, device="cuda"), torch.ones(64, device="cuda")
+    i = torch.zeros(3, dtype=torch.int32, device="cuda")
+    w = torch.zeros(2, 32, 64, dtype=BF16, device="cuda")
+    w8, h8, f8, f2 = w.to(torch.int8), h.to(torch.int8), torch.ones(8, device="cuda"), torch.ones(2, 32, device="cuda")
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    for call in (lambda: ops.block_norm(h), lambda: ops.block_norm_quant_i8(h, None, None, (f, None)),
+                 lambda: ops.rotary(h[None], i[:1], torch.ones(32, dtype=torch.float64, device="cuda")),
+                 lambda: ops.route_topk(f.reshape(8, 8), 2), lambda: ops.gemm_grouped(h, w, i),
+                 lambda: ops.gemm_i8_grouped(h8, f8, w8, f2, i), lambda: ops.combine_topk(h, i[:2].reshape(1, 2), f[:2].reshape(1, 2))):
+        with pytest.raises(RuntimeError, match="current device is cuda:1"):
+            call()
+
+
+def test_first_call_inside_a_capture_is_refused(ops, monkeypatch):
+    """The status word of a device outlives every graph: a capture may not be what allocates it."""
+    h, w = torch.zeros(8, 64, dtype=BF16, device="cuda"), torch.zeros(2, 32, 64, dtype=BF16, device="cuda")
+    i = torch.zeros(3, dtype=torch.int32, device="cuda")
+    monkeypatch.setattr(ops, "_status_words", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="before capturing"):
+        ops.gemm_grouped(h, w, i)
+
+
+def test_offsets_past_32_bits(ops):
+    """Tensors of more than 2^31 elements: the last rows are as right as the first."""
+    g = gen(2)
+    rows, C = (1 << 31) // 1280 + 7001, 1280
+    pick = torch.tensor([0, 1, rows // 2, rows - 2, rows - 1], device="cuda")
+    x = torch.empty(rows, C, dtype=BF16, device="cuda")
+    for lo in range(0, rows, 1 << 18):                   # rows of few different values, made in pieces
+        x[lo:lo + (1 << 18)] = (torch.arange(lo, min(rows, lo + (1 << 18)), device="cuda")[:, None] * 7 + torch.arange(C, device="cuda") * 3).remainder(251).to(BF16) / 64
+    pre = (rand(g, C), rand(g, C))
+    few = x[pick].contiguous()
+    a, y = ops.block_norm(x, x, post=pre, pre=pre)
+    wa, wy = ops.block_norm(few, few, post=pre, pre=pre)
+    x64, ex, y64, ey = block64(few, few, pre, pre, None, 1.0, False)
+    near(a[pick], x64, ex)
+    near(y[pick], y64, ey)
+    near(wa, x64, ex)
+    del a, y
+    # one plane of heads of 64, then of positions: rows past 2^31 / 64
+    planes = x.view(-1)[: 2 * ((1 << 30) // 64 + 64) * 64].view(2, -1, 64)
+    freqs, _ = ops.rotary_freqs(64)
+    pos = torch.arange(64, device="cuda")
+    out = ops.rotary(planes, pos, freqs)
+    assert torch.equal(out[1, -64:], ops.rotary(planes[1:, -64:].contiguous(), pos, freqs)[0])
+    assert torch.equal(out[0, :64], ops.rotary(planes[:1, :64].contiguous(), pos, freqs)[0])
+    del out, planes
+    # combination and grouped products: the last tokens choose the last rows
+    T = rows // 2
+    slots = torch.arange(2 * T, device="cuda", dtype=torch.int32).reshape(T, 2)
+    wts = torch.rand(T, 2, generator=g, device="cuda")
+    out = ops.combine_topk(x, slots, wts)
+    end = torch.tensor([T - 2, T - 1], device="cuda")
+    terms = x[slots[end].long()].double() * wts[end].double()[..., None]
+    near(out[end], terms.sum(1), 3 * U32 * terms.abs().sum(1))
+    del out
+    w = rand(g, 3, C, 64, by=0.1, t=BF16)
+    off = torch.tensor([0, 5, rows - 300, rows], dtype=torch.int32, device="cuda")
+    tall = x[:, :64]                                     # leading dimension 1280: A reaches past 2^31 elements too
+    src = torch.arange(rows - 1, -1, -1, device="cuda", dtype=torch.int32)
+    for idx in (None, src):
+        out = ops.gemm_grouped(tall, w, off, rows=idx)
+        ops.check_status()
+        e = torch.tensor([0, 1, 1, 2, 2], device="cuda")
+        at = torch.tensor([4, 5, rows // 2, rows - 300, rows - 1], device="cuda")
+        ar = tall[at if idx is None else src[at].long()].double()
+        want = torch.einsum("sk,snk->sn", ar, w[e].double())
+        near(out[at], want, 64 * 2.0 ** -23 * torch.einsum("sk,snk->sn", ar.abs(), w[e].double().abs()))
+        del out
 
 
 def test_empty_calls(ops):
