@@ -545,6 +545,9 @@ def normalize_u8(x: torch.Tensor, mean, std, out: Optional[torch.Tensor] = None)
 _F32, _F16, _BF16, _I32 = torch.float32, torch.float16, torch.bfloat16, torch.int32
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream       # the current stream of a device, as a pointer
+
+
 def _here(t: torch.Tensor, dtype: torch.dtype, dev: int, name: str) -> None:
     """``_need`` against a device number that the caller has asked for once."""
     if t.dtype is not dtype or t.get_device() != dev:
@@ -556,26 +559,25 @@ def _half(t: torch.Tensor, name: str) -> Tuple[torch.dtype, int]:
     dtype = t.dtype
     if dtype is not _BF16 and dtype is not _F16:
         raise RuntimeError(f"{name}: expected bfloat16 or float16, got {dtype}")
-    if not t.is_cuda:
+    dev = t.get_device()
+    if dev < 0 or dev != torch.cuda.current_device():
         _need(t, dtype, name)
-    dev = torch.cuda.current_device()
-    _here(t, dtype, dev, name)
     return dtype, dev
 
 
 def _vector(t: torch.Tensor, name: str, dev: int, shape: Tuple[int, ...]) -> int:
     """Pointer of a contiguous fp32 tensor of this shape."""
-    _here(t, _F32, dev, name)
-    if t.shape != shape or not t.is_contiguous():
-        raise RuntimeError(f"{name}: expected a contiguous float32 tensor of shape {list(shape)}, got {list(t.shape)}")
-    return t.data_ptr()
+    if t.dtype is _F32 and t.get_device() == dev and t.shape == shape and t.is_contiguous():
+        return t.data_ptr()
+    _need(t, _F32, name)
+    raise RuntimeError(f"{name}: expected a contiguous float32 tensor of shape {list(shape)}, got {list(t.shape)}")
 
 
 def _indexes(t: torch.Tensor, name: str, dev: int, n: int) -> int:
-    _here(t, _I32, dev, name)
-    if t.shape != (n,) or not t.is_contiguous():
-        raise RuntimeError(f"{name}: expected a contiguous int32 tensor of {n} elements, got {list(t.shape)}")
-    return t.data_ptr()
+    if t.dtype is _I32 and t.get_device() == dev and t.shape == (n,) and t.is_contiguous():
+        return t.data_ptr()
+    _need(t, _I32, name)
+    raise RuntimeError(f"{name}: expected a contiguous int32 tensor of {n} elements, got {list(t.shape)}")
 
 
 def _matrix(t: torch.Tensor, name: str) -> int:
@@ -590,10 +592,15 @@ def _matrix(t: torch.Tensor, name: str) -> int:
 
 def _like(t: torch.Tensor, dtype: torch.dtype, dev: int, shape, name: str) -> int:
     """Leading dimension of a matrix that has to have this type and shape."""
-    _here(t, dtype, dev, name)
+    if t.dtype is not dtype or t.get_device() != dev:
+        _need(t, dtype, name)
     if t.shape != shape:
         raise RuntimeError(f"{name}: expected shape {list(shape)}, got {list(t.shape)}")
-    return _matrix(t, name)
+    ld, inner = t.stride()
+    rows, cols = shape
+    if inner != 1 and cols > 1:
+        raise RuntimeError(f"{name}: expected unit inner stride")
+    return ld if rows > 1 else cols
 
 
 def _status(t: torch.Tensor, dev: int) -> int:
@@ -606,50 +613,37 @@ def _status(t: torch.Tensor, dev: int) -> int:
     return w.data_ptr()
 
 
-def _block_norm(fn: str, h, residual, post, pre, gate, res_scale, eps, rms, out, quant):
-    dtype, dev = _half(h, "h")
+def _norm_args(h, dtype, dev, residual, post, pre, gate, out):
+    """Arguments of the block norms up to the gate, the output and its leading dimension."""
     ldh = _matrix(h, "h")
     shape = h.shape
     rows, C = shape
-    pr = pgg = pgb = pqg = pqb = pg = py = ps = None
+    vec = (C,)
+    pr = pgg = pgb = pqg = pqb = pg = None
     ldr = gates = 0
     if residual is not None:
         ldr = _like(residual, dtype, dev, shape, "residual")
         pr = residual.data_ptr()
     if post is not None:
         gain, offset = post
-        pgg = _vector(gain, "post gain", dev, (C,))
+        pgg = _vector(gain, "post gain", dev, vec)
         if offset is not None:
-            pgb = _vector(offset, "post offset", dev, (C,))
+            pgb = _vector(offset, "post offset", dev, vec)
     if pre is not None:
         gain, offset = pre
-        pqg = _vector(gain, "pre gain", dev, (C,))
+        pqg = _vector(gain, "pre gain", dev, vec)
         if offset is not None:
-            pqb = _vector(offset, "pre offset", dev, (C,))
+            pqb = _vector(offset, "pre offset", dev, vec)
     if gate is not None:
         gates = gate.shape[0] if gate.dim() == 2 else 1
-        pg = _vector(gate, "gate", dev, (gates, C) if gate.dim() == 2 else (C,))
+        pg = _vector(gate, "gate", dev, (gates, C) if gate.dim() == 2 else vec)
         if gates == 0 or rows % gates:
             raise RuntimeError(f"gate: {gates} vectors do not divide {rows} rows")
     if out is None:
         out, ldx = torch.empty_like(h), C                 # rows of unit inner stride: a dense copy is row-major
     else:
         ldx = _like(out, dtype, dev, shape, "out")
-    y = scale = None
-    if quant:
-        y = torch.empty(rows, C, dtype=torch.int8, device=h.device)
-        scale = torch.empty(rows, dtype=_F32, device=h.device)
-        _lib.check(_lib.load().samb_block_norm_quant_i8(
-            h.data_ptr(), ldh, pr, ldr, pgg, pgb, pqg, pqb, pg, gates, res_scale, eps, rms, out.data_ptr(), ldx,
-            y.data_ptr(), scale.data_ptr(), rows, C, _stream()), fn)
-    else:
-        if pre is not None:
-            y = torch.empty_like(h)
-            py = y.data_ptr()
-        _lib.check(_lib.load().samb_block_norm(
-            h.data_ptr(), ldh, pr, ldr, pgg, pgb, pqg, pqb, pg, gates, res_scale, eps, dtype is _F16, rms,
-            out.data_ptr(), ldx, py, rows, C, _stream()), fn)
-    return out, y, scale
+    return (h.data_ptr(), ldh, pr, ldr, pgg, pgb, pqg, pqb, pg, gates), out, ldx
 
 
 def block_norm(h: torch.Tensor, residual: Optional[torch.Tensor] = None, post=None, pre=None,
@@ -660,7 +654,14 @@ def block_norm(h: torch.Tensor, residual: Optional[torch.Tensor] = None, post=No
     ``pre``.  ``post`` / ``pre`` are ``(gain, offset or None)`` in fp32, LayerNorm or with ``rms`` root-mean-square
     norms; ``gate`` is fp32 ``[C]``, or ``[G, C]`` with one vector for each of G equal blocks of rows.  ``out`` (x) may
     be ``residual`` or ``h``."""
-    return _block_norm("samb_block_norm", h, residual, post, pre, gate, res_scale, eps, rms, out, False)[:2]
+    dtype, dev = _half(h, "h")
+    args, x, ldx = _norm_args(h, dtype, dev, residual, post, pre, gate, out)
+    y = torch.empty_like(h) if pre is not None else None
+    rows, C = h.shape
+    _lib.check(_lib.load().samb_block_norm(*args, res_scale, eps, dtype is _F16, rms, x.data_ptr(), ldx,
+                                           None if y is None else y.data_ptr(), rows, C, _raw_stream(dev)),
+               "samb_block_norm")
+    return x, y
 
 
 def block_norm_quant_i8(h: torch.Tensor, residual: Optional[torch.Tensor], post, pre, gate: Optional[torch.Tensor] = None,
@@ -671,7 +672,14 @@ def block_norm_quant_i8(h: torch.Tensor, residual: Optional[torch.Tensor], post,
     _need(h, torch.bfloat16, "h")
     if pre is None:
         raise RuntimeError("block_norm_quant_i8 needs the norm whose output it quantises")
-    return _block_norm("samb_block_norm_quant_i8", h, residual, post, pre, gate, res_scale, eps, rms, out, True)
+    dev = h.get_device()
+    args, x, ldx = _norm_args(h, _BF16, dev, residual, post, pre, gate, out)
+    rows, C = h.shape
+    yq = torch.empty(rows, C, dtype=torch.int8, device=h.device)
+    scale = torch.empty(rows, dtype=_F32, device=h.device)
+    _lib.check(_lib.load().samb_block_norm_quant_i8(*args, res_scale, eps, rms, x.data_ptr(), ldx, yq.data_ptr(),
+                                                    scale.data_ptr(), rows, C, _raw_stream(dev)), "samb_block_norm_quant_i8")
+    return x, yq, scale
 
 
 def rotary_freqs(rot: int, base: float = 10000.0, axes: int = 1, scaling: Optional[str] = None, factor: float = 1.0,
@@ -744,7 +752,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, interl
         rs = ors = 0
     _lib.check(_lib.load().samb_rotary(
         x.data_ptr(), ps, rs, positions.data_ptr(), pt is torch.int64, period, axes, freqs.data_ptr(), 2 * freqs.shape[0],
-        interleaved, mscale, out.data_ptr(), ops_, ors, planes, rows, d, dtype is _F16, _stream()), "samb_rotary")
+        interleaved, mscale, out.data_ptr(), ops_, ors, planes, rows, d, dtype is _F16, _raw_stream(dev)), "samb_rotary")
     return out
 
 
@@ -764,10 +772,9 @@ def route_topk(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] = None
     logits (plus ``bias [E]``, which decides the choice only; ties to the lower index), their softmax or sigmoid
     weights, and the order of the choices by expert for ``gemm_grouped`` and ``combine_topk``.  An expert at -inf or NaN
     is never chosen: a token with nobody left (a padded one) gets id -1, weight 0 and no place."""
-    if logits.dtype is not _F32 or not logits.is_cuda:
+    dev = logits.get_device()
+    if logits.dtype is not _F32 or dev < 0 or dev != torch.cuda.current_device():
         _need(logits, _F32, "logits")
-    dev = torch.cuda.current_device()
-    _here(logits, _F32, dev, "logits")
     ld = _matrix(logits, "logits")
     T, E = logits.shape
     if not 1 <= k <= min(8, E):
@@ -781,7 +788,7 @@ def route_topk(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] = None
     at = buf.data_ptr()
     _lib.check(lib.samb_route_topk(
         logits.data_ptr(), ld, _vector(bias, "bias", dev, (E,)) if bias is not None else None, T, E, k, sigmoid, renorm,
-        scale, at, weights.data_ptr(), at + 4 * n, at + 8 * n, at + 12 * n, at + 4 * (3 * n + E + 1), _stream()),
+        scale, at, weights.data_ptr(), at + 4 * n, at + 8 * n, at + 12 * n, at + 4 * (3 * n + E + 1), _raw_stream(dev)),
         "samb_route_topk")
     return Routing(buf.as_strided((T, k), (k, 1), 0), weights, buf.as_strided((T, k), (k, 1), n),
                    buf.as_strided((n,), (1,), 2 * n), buf.as_strided((E + 1,), (1,), 3 * n))
@@ -828,11 +835,11 @@ def _grouped(kind, a, a_scale, w, w_scale, offsets, rows, bias, gelu, out, dtype
         _lib.check(lib.samb_gemm_i8_grouped(
             a.data_ptr(), lda, M, _vector(a_scale, "a_scale", dev, (M,)), prow, w.data_ptr(), ldw, ws,
             _vector(w_scale, "w_scale", dev, (E, N)), pbias, poff, out.data_ptr(), ldo, S, E, N, K, epi, psc, st,
-            _stream()), "samb_gemm_i8_grouped")
+            _raw_stream(dev)), "samb_gemm_i8_grouped")
     else:
         _lib.check(lib.samb_gemm_grouped(
             a.data_ptr(), lda, M, prow, w.data_ptr(), ldw, ws, pbias, poff, out.data_ptr(), ldo, S, E, N, K,
-            dtype is _F16, epi, psc, st, _stream()), "samb_gemm_grouped")
+            dtype is _F16, epi, psc, st, _raw_stream(dev)), "samb_gemm_grouped")
     return out
 
 
@@ -856,7 +863,7 @@ def gemm_i8_grouped(aq: torch.Tensor, a_scale: torch.Tensor, wq: torch.Tensor, w
     if a_scale is None or w_scale is None:
         raise RuntimeError("gemm_i8_grouped needs both scales")
     return _grouped("gemm_i8_grouped", aq, a_scale, wq, w_scale, offsets, rows, bias, gelu, out, torch.int8,
-                    torch.cuda.current_device())
+                    aq.get_device())
 
 
 def combine_topk(x: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, residual: Optional[torch.Tensor] = None,
@@ -881,5 +888,5 @@ def combine_topk(x: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, re
         ldo = _like(out, dtype, dev, (T, C), "out")
     _lib.check(_lib.load().samb_combine_topk(
         x.data_ptr(), ldx, S, slots.data_ptr(), _vector(weights, "weights", dev, (T, k)), pr, ldr, out.data_ptr(), ldo,
-        T, k, C, dtype is _F16, _stream()), "samb_combine_topk")
+        T, k, C, dtype is _F16, _raw_stream(dev)), "samb_combine_topk")
     return out
