@@ -7,7 +7,7 @@
 // after a barrier when one block is enough) it adds up the counts of the blocks before it and places its pairs in
 // order: a warp owns a run of pairs, ranks equal experts among its lanes with match_any and keeps a running count per
 // expert in shared memory.  Nothing depends on the order in which atomics arrive.  Bound by latency: 19 us for 32768 tokens x
-// 64 experts, k = 4 (34 us with a warp a token), 3.8 us for one token.
+// 64 experts, k = 4 (34 us with a warp a token, 20 us with four a warp by warp-wide maxima and ballots), 3.8 us for one token.
 #include "common.cuh"
 
 namespace samb {
@@ -304,11 +304,11 @@ route_place_kernel(const RouteParams p) {
 
 constexpr int kSmallExperts = 64;                          // eight lanes a token
 
-// One block for up to eight rounds of its warps, otherwise one a run of tokens, at most one an SM (their counts are read
-// by every block).
+// One block for up to two rounds of its warps (64 experts: 128 tokens take 8.7 us in one block and in two launches alike, 256
+// tokens 14.0 and 8.5), otherwise one a round of tokens, at most one an SM (their counts are read by every block).
 int route_blocks(int64_t T, int E) {
   const int step = kRouteWarps * (E <= kSmallExperts ? 4 : 1);
-  if (T <= 8 * step) return 1;
+  if (T <= 2 * step) return 1;
   const int64_t want = (T + step - 1) / step, most = 148;
   return int(want < most ? want : most);
 }
