@@ -8,12 +8,12 @@
 // number of tiles is what spreads their stream over the SMs; and for a handful of rows in all (serving a token or two) dot
 // products by warps, which have neither tensor maps to build nor a pipeline to fill.
 //
-// Operands: 128-byte K slabs in a ring of 128B-swizzled stages, W by TMA, and A too when its rows lie in order.  With
-// `rows` the single-CTA kernel has a warp per stage fetch them with 16-byte cp.async into the same swizzled places.  The
-// pair kernel would gather every row again for each of its column tiles, faster than cp.async delivers them (774 us
-// against 590 us for rows in order at 65536 x 5120 x 1280; TMA's own gather of four rows, at some 85 cycles an
-// instruction, took 2110 us), so large products have their rows put in order first, in caller scratch: a pass at copy
-// bandwidth (40 us there).
+// Operands: 128-byte K slabs in a ring of 128B-swizzled stages, W by TMA, and A too.  With `rows` the single-CTA kernel
+// gathers A four rows a copy (tile::gather4, four warps: within 2 to 8 % of rows in order; 16-byte cp.async into the same
+// places takes 1.5 times as long, its writes compete with the tensor core for shared memory).  The pair kernel would
+// gather every row again for each of its column tiles; there a pass at copy bandwidth that puts the rows in order first,
+// in caller scratch, is the better one (16384 x 5120 x 1280: 162 us against 160 us, but 127 against 135 us in int8, and 752
+// against 764 us at 65536 rows under the power cap).
 //
 // Measured, one B200: 65536 x 5120 x 1280 bf16 with 16 experts, gathered, bias and GELU: 650 us = 1.32 PFLOP/s (one dense
 // product of that size: 578 us here, 587 us by the vendor library); 16384 x 5120 x 1280 int8: 111 us = 1.9 POP/s; 2062 x 1280 x
@@ -40,7 +40,7 @@ enum { kTypeBf16 = 0, kTypeF16 = 1, kTypeI8 = 2 };
 
 struct GroupedParams {
   void* out;
-  const uint8_t* a;                // for the gathering warps
+  const uint8_t* a;
   const float* bias;               // [E, N] or null
   const float* a_scale;            // int8: per row of A
   const float* w_scale;            // int8: [E, N]
@@ -124,54 +124,13 @@ struct TileWalk {
   }
 };
 
-// A gathering warp owns one stage of the ring: for every STAGES-th slab it waits until the stage is free, fetches 128
-// rows of A with 32 cp.async a lane, eight lanes a row, waits for them and passes the slab on.  Rows whose index lies
-// outside A and columns behind K are filled with zeros.  cp.async writes through the generic proxy and the tensor core
-// reads through the async one; the fence between the two waits for the thread's copies in flight, so a thread with
-// several slabs in flight would pay the whole memory latency for each of them.  Here the warps overlap.
-template <int STAGES, int kStageBytes, typename Arrive>
-__device__ __forceinline__ void gather_role(const GroupedParams& p, TileWalk w, uint8_t* smem, uint64_t* empty_bar,
-                                            volatile int* abort_flag, int stage, int tile0, int step, int num_tiles,
-                                            Arrive arrive) {
-  const int lane = threadIdx.x & 31;
-  const int unit = lane & 7, quarter = lane >> 3;
-  // row 4 j + quarter goes to its 128 bytes, the 16-byte units exchanged as the 128B swizzle wants it
-  const uint32_t dst_even = smem_u32(smem) + stage * kStageBytes + quarter * 128 + ((unit ^ quarter) << 4);
-  const uint32_t dst_odd = smem_u32(smem) + stage * kStageBytes + quarter * 128 + ((unit ^ (quarter + 4)) << 4);
-  uint32_t phase = 0;
-  int slab = stage;                                      // slab of the current tile that is this warp's next
-  for (int tile = tile0; tile < num_tiles; tile += step, slab -= p.k_slabs) {
-    if (slab >= p.k_slabs) continue;
-    w.at(tile);
-    int idx[4];                                          // rows 32 i + lane of the tile
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int m = i * 32 + lane;
-      const int r = m < w.rows ? __ldg(p.rows + w.m0 + m) : -1;
-      idx[i] = r < p.a_rows ? r : -1;
-    }
-    for (; slab < p.k_slabs; slab += STAGES) {
-      if (!warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, 8)) return;
-      const int k0 = slab * SLAB_BYTES + unit * 16;
-      const bool inside = k0 < p.k_bytes;
-      const uint8_t* base = p.a + (inside ? k0 : 0);
-#pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        if (j * 4 >= w.rows) break;                     // what lies behind the tile's rows may be anything
-        const int r = __shfl_sync(0xffffffffu, idx[j >> 3], (j & 7) * 4 + quarter);
-        const bool there = inside && r >= 0;
-        const uint8_t* s = base + (there ? r : 0) * p.a_pitch;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(((j & 1) ? dst_odd : dst_even) + j * 512), "l"(s),
-                     "r"(there ? 16 : 0)
-                     : "memory");
-      }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      asm volatile("fence.proxy.async;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) arrive(stage);
-      phase ^= 1u;
-    }
-  }
+// Four rows of a 2-D tensor, 128 bytes each, into 512 consecutive (swizzled) bytes; `m` has boxes one row high.
+__device__ __forceinline__ void tma_gather4(void* smem_dst, const CUtensorMap* m, uint64_t* bar, int x, const int (&r)[4]) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+      ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(x), "r"(r[0]), "r"(r[1]),
+      "r"(r[2]), "r"(r[3])
+      : "memory");
 }
 
 // A wait gave up somewhere: the producer sees its copies in flight home before the CTA ends.
@@ -198,11 +157,12 @@ constexpr int ONE_STAGES = 4;
 constexpr int ONE_STAGE_BYTES = A_STAGE_BYTES + BN * SLAB_BYTES;
 constexpr int A_BOX_ROWS = 32;                           // up to 64 rows of A: only the boxes that hold some are loaded
 constexpr int A_BOX_BYTES = A_BOX_ROWS * SLAB_BYTES;
-constexpr int ONE_THREADS = 64 + 256;                    // producer, MMA, eight epilogue warps (and the gathering ones)
+constexpr int ONE_THREADS = 64 + 256;                    // producer, MMA, eight epilogue warps
+constexpr int GATHER_WARPS = 4, GATHER_GROUPS = BM / 4 / GATHER_WARPS;
 constexpr int ONE_SMEM_BYTES = ONE_STAGES * ONE_STAGE_BYTES + OUT_STAGE_BYTES + 2 * BN * 4 + 2 * (kMaxExperts + 1) * 4 + 1024 + 256;
 
 template <int kType, bool kGelu, bool kGather>
-__global__ void __launch_bounds__(ONE_THREADS + (kGather ? 32 * ONE_STAGES : 0), 1)
+__global__ void __launch_bounds__(ONE_THREADS + (kGather ? 32 * GATHER_WARPS : 0), 1)
 grouped_one_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA32,
                    const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmOut, const GroupedParams p) {
   constexpr bool kInt8 = kType == kTypeI8;
@@ -228,7 +188,7 @@ grouped_one_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full_bar[s], 1 + (kGather ? 1 : 0));
+      mbar_init(&full_bar[s], 1 + (kGather ? GATHER_WARPS : 0));
       mbar_init(&empty_bar[s], 1);
     }
     for (int a = 0; a < NUM_ACC; ++a) {
@@ -236,10 +196,8 @@ grouped_one_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       mbar_init(&acc_empty[a], 8);
     }
     fence_mbar_init();
-    if (!kGather) {
-      tma_prefetch_desc(&tmA);
-      tma_prefetch_desc(&tmA32);
-    }
+    tma_prefetch_desc(&tmA);
+    if (!kGather) tma_prefetch_desc(&tmA32);
     tma_prefetch_desc(&tmB);
     tma_prefetch_desc(&tmOut);
   }
@@ -286,19 +244,22 @@ grouped_one_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         if (!(ok = warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, 1))) break;
         uint8_t* sa = smem + stage * STAGE_BYTES;
         uint64_t* bar = &full_bar[stage];
-        if (lane == 0) mbar_expect_tx(bar, (kGather ? 0 : a_boxes * A_BOX_BYTES) + bn * SLAB_BYTES);
-        __syncwarp();
-        // W in pieces of 64 rows
-        if (!kGather) {
-          if (a_boxes == BM / A_BOX_ROWS) {
-            if (lane == 0) tma_load_2d(sa, &tmA, bar, ks * slab_elems, w.m0);
-          } else if (lane >= 8 && lane < 8 + a_boxes) {
-            tma_load_2d(sa + (lane - 8) * A_BOX_BYTES, &tmA32, bar, ks * slab_elems, w.m0 + (lane - 8) * A_BOX_ROWS);
+        if (elect_one()) {
+          mbar_expect_tx(bar, (kGather ? (w.rows + 3) / 4 * 512 : a_boxes * A_BOX_BYTES) + bn * SLAB_BYTES);
+          if (!kGather) {
+            if (a_boxes == BM / A_BOX_ROWS) {
+              tma_load_2d(sa, &tmA, bar, ks * slab_elems, w.m0);
+            } else {
+              tma_load_2d(sa, &tmA32, bar, ks * slab_elems, w.m0);
+              if (a_boxes == 2) tma_load_2d(sa + A_BOX_BYTES, &tmA32, bar, ks * slab_elems, w.m0 + A_BOX_ROWS);
+            }
           }
+#pragma unroll
+          for (int b = 0; b < BN / 64; ++b)
+            if (b * 64 < bn)
+              tma_load_3d(sa + A_STAGE_BYTES + b * (64 * SLAB_BYTES), &tmB, bar, ks * slab_elems, n0 + b * 64, w.e);
         }
         __syncwarp();
-        if (lane < bn / 64)
-          tma_load_3d(sa + A_STAGE_BYTES + lane * (64 * SLAB_BYTES), &tmB, bar, ks * slab_elems, n0 + lane * 64, w.e);
         ++issued;
         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
       }
@@ -341,8 +302,39 @@ grouped_one_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     }
   } else if (kGather && warp >= ONE_THREADS / 32) {
     // ------------------------------------------------------------------ gathering warps
-    gather_role<STAGES, STAGE_BYTES>(p, w, smem, empty_bar, abort_flag, warp - ONE_THREADS / 32, int(blockIdx.x),
-                                     int(gridDim.x), num_tiles, [&](int s) { mbar_arrive(&full_bar[s]); });
+    // Warp g fetches the rows 4 (4 j + g) .. + 3 of the tile for every slab.  Their indexes are spread over the warp's
+    // registers once a tile: the copy takes them from uniform registers, and shuffling them there for every slab, or
+    // one lane a copy, made a copy cost 60 to 85 cycles of issue.
+    const int g = warp - ONE_THREADS / 32;
+    uint32_t stage = 0, phase = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
+      w.at(tile);
+      int mine[4], r[GATHER_GROUPS][4];                  // lane j: the rows of group j
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int m = ((lane & (GATHER_GROUPS - 1)) * GATHER_WARPS + g) * 4 + q;
+        const int i = m < w.rows ? __ldg(p.rows + w.m0 + m) : 0;
+        mine[q] = i >= 0 && i < p.a_rows ? i : 0;        // outside A: any row, the epilogue drops its product
+      }
+#pragma unroll
+      for (int j = 0; j < GATHER_GROUPS; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) r[j][q] = __shfl_sync(0xffffffffu, mine[q], j);
+      for (int ks = 0; ks < p.k_slabs; ++ks) {
+        if (!(ok = warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, 8))) break;
+        uint8_t* sa = smem + stage * STAGE_BYTES + g * 512;
+        if (elect_one()) {
+#pragma unroll
+          for (int j = 0; j < GATHER_GROUPS; ++j)
+            if ((j * GATHER_WARPS + g) * 4 < w.rows)
+              tma_gather4(sa + j * (GATHER_WARPS * 512), &tmA, &full_bar[stage], ks * slab_elems, r[j]);
+          mbar_arrive(&full_bar[stage]);                 // a warp without rows must not fall behind either
+        }
+        __syncwarp();
+        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+      }
+    }
   } else {
     // ------------------------------------------------------------------ epilogue
     const uint32_t lane_base = uint32_t(warp & 3) * 32u;
@@ -360,9 +352,11 @@ grouped_one_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         if (kInt8) s_wscale[et] = inside ? __ldg(p.w_scale + (long long)w.e * p.N + n) : 0.f;
       }
       float a_scale = 1.f;
-      if (kInt8 && erow < w.rows) {
+      bool there = true;                                 // this row's index points into A (else: a row of zeros)
+      if ((kGather || kInt8) && erow < w.rows) {
         const int i = p.rows != nullptr ? __ldg(p.rows + w.m0 + erow) : w.m0 + erow;
-        if (i >= 0 && i < p.a_rows) a_scale = __ldg(p.a_scale + i);        // else: a row of zeros, whatever its scale
+        there = i >= 0 && i < p.a_rows;
+        if (kInt8 && there) a_scale = __ldg(p.a_scale + i);
       }
       const bool got = mbar_wait(&acc_full[acc], acc_phase, abort_flag, p.status, 4);
       if (!epi_all(got)) break;                          // also publishes the column vectors
@@ -376,6 +370,10 @@ grouped_one_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         uint32_t r[32];
         tmem_ld_32x32b_x32(t_addr + c * 64, r);
         tmem_ld_wait();
+        if (kGather && !there) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) r[j] = 0u;
+        }
         uint4 packed[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -903,11 +901,6 @@ PairFn pair_kernel(int type, bool bias, bool gelu) {
 constexpr int64_t kPairRows = 512;
 bool want_pairs(int64_t S, int E) { return S >= kPairRows * int64_t(E); }
 
-// Gathered rows are put in order first from 32 rows an expert, when a row has 1 KB at least (16 experts, 5120 x 1280 bf16,
-// in the kernel against a pass first: 41 / 41 us at 16 rows an expert, 46 / 42 at 32, 56 / 48 at 64, 69 / 48 at 128; 64
-// experts, 512 x 256: 10.9 / 12.3 at 16, 15.1 / 15.8 at 128), and always for pairs.
-bool want_order(int64_t S, int E, int64_t row_bytes) { return want_pairs(S, E) || (S >= 32 * int64_t(E) && row_bytes >= 1024); }
-
 int launch_pairs(int type, bool gelu, const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmOut,
                  const GroupedParams& p, cudaStream_t st) {
   const bool int8 = type == kTypeI8;
@@ -1014,7 +1007,7 @@ int launch_grouped(int type, const void* A, int64_t lda, int64_t a_rows, const f
     return launch_status();
   }
   // what the products read: A itself, or its rows in order in the caller's scratch
-  const bool order = gather && scratch != nullptr && want_order(S, E, p.k_bytes);
+  const bool order = gather && scratch != nullptr && want_pairs(S, E);
   const void* from = order ? scratch : A;
   const int64_t from_ld = order ? K : lda, from_rows = order ? S : a_rows;
   if (order) {
@@ -1023,7 +1016,7 @@ int launch_grouped(int type, const void* A, int64_t lda, int64_t a_rows, const f
     order_rows_kernel<<<unsigned(blocks), 256, 0, st>>>(p, static_cast<uint4*>(scratch));
     if (int e = launch_status()) return e;
   }
-  if (int e = map_a(&tmA, from, from_ld, from_rows, BM)) return e;
+  if (int e = map_a(&tmA, from, from_ld, from_rows, gather && !order ? 1 : BM)) return e;
   // the pair kernel's epilogue reads the column vectors in 16-byte pieces; it wants its rows in order
   if (want_pairs(S, E) && (!gather || order) &&
       !((reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(w_scale)) & 15u)) {
@@ -1039,7 +1032,7 @@ int launch_grouped(int type, const void* A, int64_t lda, int64_t a_rows, const f
     return SAMB_E_LAUNCH;
   const long long most = ((S + BM - 1) / BM + E) * ((N + 63) / 64);
   const unsigned grid = unsigned(most < sm_count() ? most : sm_count());
-  kern<<<grid, ONE_THREADS + (in_kernel ? 32 * ONE_STAGES : 0), ONE_SMEM_BYTES, st>>>(tmA, tmA32, tmB, tmOut, p);
+  kern<<<grid, ONE_THREADS + (in_kernel ? 32 * GATHER_WARPS : 0), ONE_SMEM_BYTES, st>>>(tmA, tmA32, tmB, tmOut, p);
   return launch_status();
 }
 
@@ -1049,8 +1042,7 @@ int launch_grouped(int type, const void* A, int64_t lda, int64_t a_rows, const f
 extern "C" {
 
 int64_t samb_gemm_grouped_scratch_bytes(int64_t S, int E, int K, int is_i8) {
-  const int64_t row = int64_t(K) * (is_i8 ? 1 : 2);
-  return S > samb::kFewSlots && E > 0 && K > 0 && samb::want_order(S, E, row) ? S * row : 0;
+  return S > samb::kFewSlots && E > 0 && K > 0 && samb::want_pairs(S, E) ? S * K * (is_i8 ? 1 : 2) : 0;
 }
 
 int samb_gemm_grouped(const void* A, int64_t lda, int64_t a_rows, const int32_t* rows, const void* W, int64_t ldw,

@@ -737,13 +737,12 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, interl
     if freqs.dim() != 1 or not freqs.is_contiguous():
         raise RuntimeError("freqs: expected a contiguous 1-D tensor")
     if out is None:
-        out = torch.empty(planes, rows, d, dtype=dtype, device=x.device)
-        ops_, ors, oes = rows * d, d, 1
+        out = torch.empty_like(x)                         # laid out like x where x has no gaps
     else:
         _here(out, dtype, dev, "out")
         if out.shape != x.shape:
             raise RuntimeError("out must have the shape of x")
-        ops_, ors, oes = out.stride()
+    ops_, ors, oes = out.stride()
     if d > 1 and (es != 1 or oes != 1):
         raise RuntimeError("x and out: expected unit inner stride")
     if planes <= 1:                                       # strides of a single plane or row mean nothing
@@ -781,15 +780,15 @@ def route_topk(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] = None
         raise RuntimeError(f"k: {k} is not between 1 and 8 and at most the number of experts ({E})")
     lib = _lib.load()
     n = T * k
-    scratch = lib.samb_route_scratch_bytes(T, E) // 4
-    # one allocation for the whole numbers: ids, slots, rows, offsets, scratch
-    buf = torch.empty(3 * n + E + 1 + scratch, dtype=_I32, device=logits.device)
+    pbias = None if bias is None else _vector(bias, "bias", dev, (E,))
+    room = lib.samb_route_scratch_bytes(T, E) // 4
+    # one allocation for the whole numbers: ids, slots, rows, offsets and the scratch
+    buf = torch.empty(3 * n + E + 1 + room, dtype=_I32, device=logits.device)
     weights = torch.empty(T, k, dtype=_F32, device=logits.device)
     at = buf.data_ptr()
     _lib.check(lib.samb_route_topk(
-        logits.data_ptr(), ld, _vector(bias, "bias", dev, (E,)) if bias is not None else None, T, E, k, sigmoid, renorm,
-        scale, at, weights.data_ptr(), at + 4 * n, at + 8 * n, at + 12 * n, at + 4 * (3 * n + E + 1), _raw_stream(dev)),
-        "samb_route_topk")
+        logits.data_ptr(), ld, pbias, T, E, k, sigmoid, renorm, scale, at, weights.data_ptr(), at + 4 * n, at + 8 * n,
+        at + 12 * n, at + 4 * (3 * n + E + 1), _raw_stream(dev)), "samb_route_topk")
     return Routing(buf.as_strided((T, k), (k, 1), 0), weights, buf.as_strided((T, k), (k, 1), n),
                    buf.as_strided((n,), (1,), 2 * n), buf.as_strided((E + 1,), (1,), 3 * n))
 
@@ -883,7 +882,8 @@ def combine_topk(x: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, re
         ldr = _like(residual, dtype, dev, (T, C), "residual")
         pr = residual.data_ptr()
     if out is None:
-        out, ldo = torch.empty(T, C, dtype=dtype, device=x.device), C
+        out = torch.empty(T, C, dtype=dtype, device=x.device) if residual is None else torch.empty_like(residual)
+        ldo = C
     else:
         ldo = _like(out, dtype, dev, (T, C), "out")
     _lib.check(_lib.load().samb_combine_topk(

@@ -144,7 +144,7 @@ def test_rotary_freqs():
 
 def test_grouped_scratch(lib):
     f = lib.samb_gemm_grouped_scratch_bytes
-    assert f(2, 16, 1280, 0) == f(0, 1, 64, 0) == f(8, 1, 1280, 0) == f(31 * 16, 16, 1280, 0) == f(64 * 16, 16, 256, 0) == 0
+    assert f(2, 16, 1280, 0) == f(0, 1, 64, 0) == f(8, 1, 1280, 0) == f(511 * 16, 16, 1280, 0) == 0
     assert f(65536, 16, 1280, 0) == 65536 * 1280 * 2 and f(1 << 30, 8, 5120, 1) == 5120 << 30
 
 

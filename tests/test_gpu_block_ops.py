@@ -75,7 +75,8 @@ def block64(h, r, post, pre, gate, a, rms):
 
 @pytest.mark.parametrize("t,rms", [(BF16, False), (BF16, True), (F16, False), (F16, True)])
 @pytest.mark.parametrize("rows,C,gates", [(1, 8, 0), (1, 1280, 1), (3, 256, 3), (5, 264, 0), (7, 1280, 7), (130, 200, 2), (1031, 768, 1),
-                                          (6000, 1280, 6), (2376, 2048, 24), (2, 2056, 2), (300, 4104, 3), (151, 8192, 0)])
+                                          (6000, 1280, 6), (2376, 2048, 24), (2, 2056, 2), (300, 4104, 3), (151, 8192, 0),
+                                          (60000, 64, 8), (39999, 256, 3), (30011, 264, 1)])
 def test_block_norm(ops, rows, C, gates, t, rms):
     g = gen(rows * 7 + C)
     h, r = rand(g, rows, C, at=0.3, t=t), rand(g, rows, C, by=3.0, t=t)
@@ -196,7 +197,7 @@ def rotary64(x, positions, freqs, interleaved, mscale):
 @pytest.mark.parametrize("planes,rows,d,rot,axes,period,far", [
     (1, 1, 8, 2, 1, 1, 0), (32, 1, 80, 80, 1, 1, 1000000), (4, 64, 64, 64, 2, 64, 64), (3, 35, 80, 80, 2, 7, 300),
     (2, 130, 80, 40, 1, 130, 4096), (5, 33, 128, 36, 2, 11, 77), (7, 12, 24, 22, 1, 4, 50000), (2, 9, 16, 16, 1, 9, 1 << 40),
-    (1, 3000, 256, 128, 1, 1000, 1 << 30), (40, 17, 32, 4, 2, 17, 5)])
+    (1, 3000, 256, 128, 1, 1000, 1 << 30), (40, 17, 32, 4, 2, 17, 5), (1, 70000, 16, 8, 1, 1, 9), (3, 5000, 24, 24, 1, 2, 31)])
 def test_rotary(ops, planes, rows, d, rot, axes, period, far, interleaved, t):
     g = gen(planes * 31 + rows + rot)
     x = rand(g, planes, rows, d, t=t)
@@ -288,7 +289,7 @@ def check_route(ops, x, k, bias=None, sigmoid=False, renorm=True, scale=1.0):
 
 
 @pytest.mark.parametrize("sigmoid,renorm", [(False, True), (False, False), (True, True), (True, False)])
-@pytest.mark.parametrize("T,E,k", [(1, 1, 1), (1, 16, 2), (2, 3, 3), (31, 33, 8), (128, 64, 4), (129, 64, 4), (1000, 130, 6),
+@pytest.mark.parametrize("T,E,k", [(1, 1, 1), (1, 16, 2), (2, 3, 3), (31, 33, 8), (128, 64, 4), (129, 64, 4), (32, 65, 3), (33, 65, 3), (1000, 130, 6),
                                    (2369, 8, 2), (5000, 512, 8), (40000, 16, 1)])
 def test_route(ops, T, E, k, sigmoid, renorm):
     g = gen(T + E)
@@ -319,6 +320,8 @@ def test_route_strided_and_empty(ops):
     r, want = ops.route_topk(wide[:, 16:48], 2), ops.route_topk(wide[:, 16:48].contiguous(), 2)
     for a, b in zip(r, want):
         assert torch.equal(a, b)
+    r.ids.fill_(5)                                       # the results are ordinary tensors, apart from one another
+    assert torch.equal(r.slots, want.slots) and torch.equal(r.rows, want.rows) and torch.equal(r.offsets, want.offsets)
     r = ops.route_topk(wide[:0, :8], 2)
     assert r.ids.shape == (0, 2) and r.rows.numel() == 0 and r.offsets.tolist() == [0] * 9
 
@@ -379,7 +382,7 @@ CASES = [  # counts of the experts, rows behind the last, N, K, padded strides
     ([0, 0, 300, 0], 5, 520, 64, 0), ([5, 260, 1, 0, 64], 0, 72, 144, 1), ([1] * 33, 2, 64, 96, 0), ([3] * 300, 0, 40, 32, 0),
     ([700, 11, 90], 0, 1280, 1280, 0), ([1] * 8, 0, 1280, 5120, 0), ([8, 0, 3], 1, 640, 1296, 1), ([2] * 16, 0, 2560, 256, 0),
     ([4000, 3000, 1192], 0, 512, 128, 0), ([1500, 3, 257], 0, 520, 144, 1), ([2000, 0], 7, 264, 80, 0), ([600], 0, 8, 16, 0),
-    ([100, 40, 0, 200], 0, 256, 1040, 0)]
+    ([100, 40, 0, 200], 0, 256, 1040, 0), ([0] * 250 + [3] + [0] * 200 + [2] + [0] * 58, 1, 264, 64, 0), ([2, 0, 1] * 170 + [1, 1], 3, 40, 32, 0)]
 
 
 @pytest.mark.parametrize("t", [BF16, F16, torch.int8])
@@ -410,7 +413,7 @@ def test_gemm_grouped(ops, counts, behind, N, K, pad, gather, t):
 @pytest.mark.parametrize("S,K", [(6, 64), (200, 64), (200, 1024), (2400, 1024)])
 def test_gemm_grouped_bad_indexes(ops, S, K, t):
     """Indexes outside A are rows of zeros; offsets outside the buffer or falling back reach nothing outside.  (Warp dot
-    products, rows gathered in the kernel, put in order first, and on CTA pairs.)"""
+    products, rows gathered in the kernel, and put in order first for CTA pairs.)"""
     g = gen(S)
     a, w, sa, sw = operands(g, t, 50, 4, 136, K)
     rows = torch.randint(0, 50, (S,), generator=g, device="cuda", dtype=torch.int32)
