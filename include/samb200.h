@@ -395,10 +395,10 @@ int samb_route_topk(const float* logits, int64_t ld, const float* bias, int64_t 
  * are clamped, and an expert whose range falls back behind an earlier one's is empty.  Rows of out outside every range
  * are left as they were.  rows (may be null; then a_rows >= S): an index outside [0, a_rows) stands for a row of
  * zeros.  epilogue: SAMB_EPI_BIAS (bias fp32 [E, N]) and / or SAMB_EPI_GELU.
- * scratch: samb_gemm_grouped_scratch_bytes bytes (0 below 512 rows an expert), 16-byte aligned, any contents, used with
+ * scratch: samb_gemm_grouped_scratch_bytes bytes (0 but for large products), 16-byte aligned, any contents, used with
  * rows only: large products put the rows in order there first.  Null is allowed and slower.  Calls that may overlap on the GPU
  * need one each. */
-int64_t samb_gemm_grouped_scratch_bytes(int64_t S, int E, int K, int is_i8);
+int64_t samb_gemm_grouped_scratch_bytes(int64_t S, int E, int N, int K, int is_i8);
 int samb_gemm_grouped(const void* A, int64_t lda, int64_t a_rows, const int32_t* rows, const void* W, int64_t ldw,
                       int64_t w_stride, const float* bias, const int32_t* offsets, void* out, int64_t ldo, int64_t S,
                       int E, int N, int K, int is_f16, int epilogue, void* scratch, int32_t* status, void* stream);

@@ -68,7 +68,7 @@ SIGNATURES = {
     "samb_route_topk": (c_int, [_P, c_int64, _P, c_int64, c_int, c_int, c_int, c_int, c_float, _P, _P, _P, _P, _P, _P, _P]),
     "samb_gemm_grouped": (c_int, [_P, c_int64, c_int64, _P, _P, c_int64, c_int64, _P, _P, _P, c_int64, c_int64, c_int, c_int,
                                   c_int, c_int, c_int, _P, _P, _P]),
-    "samb_gemm_grouped_scratch_bytes": (c_int64, [c_int64, c_int, c_int, c_int]),
+    "samb_gemm_grouped_scratch_bytes": (c_int64, [c_int64, c_int, c_int, c_int, c_int]),
     "samb_gemm_i8_grouped": (c_int, [_P, c_int64, c_int64, _P, _P, _P, c_int64, c_int64, _P, _P, _P, _P, c_int64, c_int64,
                                      c_int, c_int, c_int, c_int, _P, _P, _P]),
     "samb_combine_topk": (c_int, [_P, c_int64, c_int64, _P, _P, _P, c_int64, _P, c_int64, c_int64, c_int, c_int, c_int, _P]),

@@ -3,8 +3,8 @@
 // The offsets live on the device (the router wrote them), so the host launches one wave of persistent CTAs and every
 // CTA works the tile list out for itself: the prefix over the experts of their row tiles, times the column tiles.
 //
-// Three kernels.  On CTA pairs (256 x 256 tiles, cta_group::2, each CTA loads its 128 rows of A and half of W) for groups
-// of some 500 rows and more; on single CTAs (128 rows, 64 to 256 columns) below, where the weights' bytes count and the
+// Three kernels.  On CTA pairs (256 x 256 tiles, cta_group::2, each CTA loads its 128 rows of A and half of W) for large
+// products of some 500 rows an expert and more; on single CTAs (128 rows, 64 to 256 columns) below, where the weights' bytes count and the
 // number of tiles is what spreads their stream over the SMs; and for a handful of rows in all (serving a token or two) dot
 // products by warps, which have neither tensor maps to build nor a pipeline to fill.
 //
@@ -896,10 +896,25 @@ PairFn pair_kernel(int type, bool bias, bool gelu) {
   return type == kTypeBf16 ? pair_of<kTypeBf16>(bias, gelu) : type == kTypeF16 ? pair_of<kTypeF16>(bias, gelu) : pair_of<kTypeI8>(bias, gelu);
 }
 
-// Pairs from 512 rows an expert.  16 experts, us, single CTAs against pairs: 5120 x 1280 bf16: 70 / 73 at 256 rows, 91 / 92
-// at 384, 112 / 103 at 512; 1280 x 5120: 74 / 70, 86 / 94, 114 / 107; 5120 x 1280 int8: 39 / 42, 47 / 49, 57 / 58.
-constexpr int64_t kPairRows = 512;
-bool want_pairs(int64_t S, int E) { return S >= kPairRows * int64_t(E); }
+// When CTA pairs are the faster kernel for rows in order: from 512 rows an expert (int8: 1024; the last tile of an expert is
+// half empty on average), two waves of tiles, and for 16-bit operands 1 KB of K (eight slabs; a short product is bound by
+// its epilogue, where the int8 pair kernel's sixteen warps win all the same).  us, single CTAs / pairs.  bf16, K 1280: 16 experts
+// 5120 wide at 256 rows an expert 70 / 73, at 384 91 / 92, at 512 112 / 103; 8 experts 1280 wide at 512 (80 tiles) 20.2 / 20.2, at
+// 1024 (160 tiles) 29.6 / 27.2, at 4096 86 / 78; 32 experts 512 wide at 512 (128 tiles) 26.2 / 29.9, at 1024 44.5 / 40.1.  bf16, 8
+// experts 1280 wide at 4096: K 512 41.6 / 39.7, K 256 34.8 / 34.2, K 128 30.0 / 32.0.  int8, there: K 128 36.3 / 28.6, K 1280 47.3 / 43.7;
+// 5120 wide, K 1280 at 512 32.5 / 35.3, at 1024 51.5 / 47.3.
+bool want_pairs(int64_t S, int E, int N, int64_t row_bytes, bool int8) {
+  const int64_t tiles = (S / (2 * BM)) * ((N + BN - 1) / BN);
+  return S >= (int8 ? 1024 : 512) * int64_t(E) && tiles >= 148 && (int8 || row_bytes >= 1024);
+}
+
+// The same for gathered rows, which pairs want in order first: the pass is worth it from some 2000 columns and eight waves.
+// us, gathered on single CTAs / in order first for pairs.  8 experts, K 1280, bf16: 1280 wide at 4096 rows an expert 96 / 101; 5120
+// wide at 512 (320 tiles) 58 / 54, at 1024 101 / 91, at 4096 371 / 318; int8: 1280 wide 57 / 59; 5120 wide 35 / 40, 62 / 53, 194 / 154.
+bool want_order(int64_t S, int E, int N, int64_t row_bytes, bool int8) {
+  const int64_t tiles = (S / (2 * BM)) * ((N + BN - 1) / BN);
+  return want_pairs(S, E, N, row_bytes, int8) && N >= 2048 && tiles >= 592;
+}
 
 int launch_pairs(int type, bool gelu, const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmOut,
                  const GroupedParams& p, cudaStream_t st) {
@@ -1007,7 +1022,8 @@ int launch_grouped(int type, const void* A, int64_t lda, int64_t a_rows, const f
     return launch_status();
   }
   // what the products read: A itself, or its rows in order in the caller's scratch
-  const bool order = gather && scratch != nullptr && want_pairs(S, E);
+  const bool int8 = type == kTypeI8;
+  const bool order = gather && scratch != nullptr && want_order(S, E, N, p.k_bytes, int8);
   const void* from = order ? scratch : A;
   const int64_t from_ld = order ? K : lda, from_rows = order ? S : a_rows;
   if (order) {
@@ -1018,7 +1034,7 @@ int launch_grouped(int type, const void* A, int64_t lda, int64_t a_rows, const f
   }
   if (int e = map_a(&tmA, from, from_ld, from_rows, gather && !order ? 1 : BM)) return e;
   // the pair kernel's epilogue reads the column vectors in 16-byte pieces; it wants its rows in order
-  if (want_pairs(S, E) && (!gather || order) &&
+  if (want_pairs(S, E, N, p.k_bytes, int8) && (!gather || order) &&
       !((reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(w_scale)) & 15u)) {
     if (int e = map_w(BN / 2)) return e;
     const int e = launch_pairs(type, gelu, tmA, tmB, tmOut, p, st);
@@ -1041,8 +1057,10 @@ int launch_grouped(int type, const void* A, int64_t lda, int64_t a_rows, const f
 
 extern "C" {
 
-int64_t samb_gemm_grouped_scratch_bytes(int64_t S, int E, int K, int is_i8) {
-  return S > samb::kFewSlots && E > 0 && K > 0 && samb::want_pairs(S, E) ? S * K * (is_i8 ? 1 : 2) : 0;
+int64_t samb_gemm_grouped_scratch_bytes(int64_t S, int E, int N, int K, int is_i8) {
+  if (S <= 0 || E <= 0 || N <= 0 || K <= 0) return 0;
+  const int64_t row = int64_t(K) * (is_i8 ? 1 : 2);
+  return samb::want_order(S, E, N, row, is_i8 != 0) ? S * row : 0;
 }
 
 int samb_gemm_grouped(const void* A, int64_t lda, int64_t a_rows, const int32_t* rows, const void* W, int64_t ldw,

@@ -813,7 +813,7 @@ def _grouped(kind, a, a_scale, w, w_scale, offsets, rows, bias, gelu, out, dtype
     if rows is not None:
         S = rows.shape[0]
         prow = _indexes(rows, "rows", dev, S)
-        room = lib.samb_gemm_grouped_scratch_bytes(S, E, K, int8)
+        room = lib.samb_gemm_grouped_scratch_bytes(S, E, N, K, int8)
         if room:                                          # room to put the rows of a large product in order
             scratch = torch.empty(room, dtype=torch.uint8, device=a.device)
             psc = scratch.data_ptr()

@@ -144,8 +144,8 @@ def test_rotary_freqs():
 
 def test_grouped_scratch(lib):
     f = lib.samb_gemm_grouped_scratch_bytes
-    assert f(2, 16, 1280, 0) == f(0, 1, 64, 0) == f(8, 1, 1280, 0) == f(511 * 16, 16, 1280, 0) == 0
-    assert f(65536, 16, 1280, 0) == 65536 * 1280 * 2 and f(1 << 30, 8, 5120, 1) == 5120 << 30
+    assert f(2, 16, 5120, 1280, 0) == f(0, 1, 5120, 64, 0) == f(511 * 16, 16, 5120, 1280, 0) == f(65536, 16, 1280, 5120, 0) == 0
+    assert f(65536, 16, 5120, 1280, 0) == 65536 * 1280 * 2 and f(1 << 30, 8, 5120, 5120, 1) == 5120 << 30
 
 
 def test_route_scratch(lib):

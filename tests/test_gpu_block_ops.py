@@ -381,7 +381,8 @@ CASES = [  # counts of the experts, rows behind the last, N, K, padded strides
     ([1], 0, 8, 16, 0), ([1, 1], 0, 256, 64, 0), ([0, 2, 0, 1, 0], 3, 264, 80, 0), ([127, 128, 129], 0, 256, 320, 0),
     ([0, 0, 300, 0], 5, 520, 64, 0), ([5, 260, 1, 0, 64], 0, 72, 144, 1), ([1] * 33, 2, 64, 96, 0), ([3] * 300, 0, 40, 32, 0),
     ([700, 11, 90], 0, 1280, 1280, 0), ([1] * 8, 0, 1280, 5120, 0), ([8, 0, 3], 1, 640, 1296, 1), ([2] * 16, 0, 2560, 256, 0),
-    ([4000, 3000, 1192], 0, 512, 128, 0), ([1500, 3, 257], 0, 520, 144, 1), ([2000, 0], 7, 264, 80, 0), ([600], 0, 8, 16, 0),
+    ([4000, 3000, 1192], 0, 1288, 128, 0), ([9000, 3, 4570], 5, 1032, 528, 1), ([20000, 0], 7, 520, 512, 0), ([600], 0, 8, 16, 0),
+    ([9000, 7001, 0, 700], 9, 2568, 528, 0),
     ([100, 40, 0, 200], 0, 256, 1040, 0), ([0] * 250 + [3] + [0] * 200 + [2] + [0] * 58, 1, 264, 64, 0), ([2, 0, 1] * 170 + [1, 1], 3, 40, 32, 0)]
 
 
@@ -410,15 +411,15 @@ def test_gemm_grouped(ops, counts, behind, N, K, pad, gather, t):
 
 
 @pytest.mark.parametrize("t", [BF16, torch.int8])
-@pytest.mark.parametrize("S,K", [(6, 64), (200, 64), (200, 1024), (2400, 1024)])
-def test_gemm_grouped_bad_indexes(ops, S, K, t):
+@pytest.mark.parametrize("S,N,K", [(6, 136, 64), (200, 136, 64), (2400, 136, 1024), (16400, 2568, 1024)])
+def test_gemm_grouped_bad_indexes(ops, S, N, K, t):
     """Indexes outside A are rows of zeros; offsets outside the buffer or falling back reach nothing outside.  (Warp dot
     products, rows gathered in the kernel, and put in order first for CTA pairs.)"""
     g = gen(S)
-    a, w, sa, sw = operands(g, t, 50, 4, 136, K)
+    a, w, sa, sw = operands(g, t, 50, 4, N, K)
     rows = torch.randint(0, 50, (S,), generator=g, device="cuda", dtype=torch.int32)
     rows[1], rows[3], rows[4] = -1, 50, 2 ** 31 - 1
-    bias = rand(g, 4, 136)
+    bias = rand(g, 4, N)
     off = torch.tensor([0, 2, 2, 5, S], dtype=torch.int32, device="cuda")
     got = call_grouped(ops, a, w, sa, sw, off, rows=rows, bias=bias)
     want, slack, written = grouped64(a, w, off, rows, bias, False, S, sa, sw)
@@ -435,10 +436,10 @@ def test_gemm_grouped_without_scratch_and_with_an_odd_bias(ops, t):
     """A product large enough for CTA pairs whose caller has no scratch, or whose bias starts at an odd place."""
     from segment_anything_fast_b200 import _lib
     g = gen(12)
-    S, M, E, N, K = 1700, 700, 3, 264, 160
+    S, M, E, N, K = 17000, 700, 3, 2568, 1024
     a, w, sa, sw = operands(g, t, M, E, N, K)
     rows = torch.randint(0, M, (S,), generator=g, device="cuda", dtype=torch.int32)
-    off = torch.tensor([0, 400, 1200, 1690], dtype=torch.int32, device="cuda")
+    off = torch.tensor([0, 4000, 12000, 16990], dtype=torch.int32, device="cuda")
     bias = rand(g, E * N + 1)[1:].reshape(E, N)
     want, slack, written = grouped64(a, w, off, rows, bias, True, S, sa, sw)
     got = call_grouped(ops, a, w, sa, sw, off, rows=rows, bias=bias, gelu=True)
