@@ -133,11 +133,13 @@ __device__ __forceinline__ void tma_gather4(void* smem_dst, const CUtensorMap* m
       : "memory");
 }
 
-// A wait gave up somewhere: the producer sees its copies in flight home before the CTA ends.
+// A wait gave up somewhere: the producer sees its copies in flight home before the CTA ends.  Those whose barrier will
+// not complete any more (a partner stopped in between) get a tenth of a millisecond, many times what a copy takes.
 template <int STAGES>
 __device__ __forceinline__ void drain_copies(uint64_t* full_bar, uint32_t issued) {
   for (uint32_t i = issued > STAGES ? issued - STAGES : 0u; i < issued; ++i)
     for (uint32_t n = 0; n < 4096u && !mbar_try_wait(&full_bar[i % STAGES], (i / STAGES) & 1u); ++n) __nanosleep(64);
+  for (int n = 0; n < 100; ++n) __nanosleep(1000);
 }
 
 __device__ __forceinline__ bool epi_all(bool pred) {
@@ -676,7 +678,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 0 && lane == 0 && rank == 0 && *abort_flag) drain_copies<STAGES>(full_bar, issued);
+  if (warp == 0 && lane == 0 && *abort_flag) drain_copies<STAGES>(full_bar, rank == 0 ? issued : 0u);
   cluster_sync_all();                                    // no CTA leaves while its peer may still signal it
   if (warp == 1) {
     tc_fence_after();

@@ -106,6 +106,30 @@ def test_combine_refusals(lib, want, change):
     assert _combine(lib, **change) == want
 
 
+def test_argument_types_match_the_header():
+    """Every argument of every function, as the header declares it, against the ctypes table."""
+    import ctypes
+    import os
+    import re
+    from segment_anything_fast_b200 import _lib
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    text = re.sub(r"/\*.*?\*/", "", open(os.path.join(root, "include", "samb200.h")).read(), flags=re.S)
+    plain = {"int": ctypes.c_int, "int32_t": ctypes.c_int32, "uint32_t": ctypes.c_uint32, "int64_t": ctypes.c_int64,
+             "float": ctypes.c_float}
+    seen = 0
+    for name, args in re.findall(r"\b(samb_[a-z0-9_]+)\s*\(([^)]*)\)", text):
+        want = [] if args.strip() == "void" else [a.strip() for a in args.split(",")]
+        have = _lib.SIGNATURES[name][1]
+        assert len(want) == len(have), name
+        for w, h in zip(want, have):
+            if "*" in w:
+                assert h is ctypes.c_void_p or issubclass(h, ctypes._Pointer), (name, w)
+            else:
+                assert h is plain[w.replace("const ", "").split()[0]], (name, w)
+        seen += 1
+    assert seen == len(_lib.SIGNATURES)
+
+
 def test_wrappers_refuse_cpu_tensors():
     from segment_anything_fast_b200 import ops
     h = torch.zeros(4, 64, dtype=torch.bfloat16)

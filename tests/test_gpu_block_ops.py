@@ -459,6 +459,47 @@ def test_gemm_grouped_without_scratch_and_with_an_odd_bias(ops, t):
     ops.check_status()
 
 
+@pytest.mark.parametrize("t", [BF16, torch.int8])
+@pytest.mark.parametrize("S,N", [(6, 264), (700, 264), (20000, 2568)])
+def test_gemm_grouped_captured_and_on_two_streams(ops, S, N, t):
+    """Each kernel (warp dot products, single CTAs with gathered rows, ordered rows on CTA pairs) in two graphs replayed in
+    turn over changing inputs, and in calls that overlap on two streams."""
+    g = gen(S)
+    E, K, M = 3, 512, 900
+    a, w, sa, sw = operands(g, t, M, E, N, K)
+    alt = [torch.flip(a, (0,)).contiguous(), a]
+    rows = [torch.randint(0, M, (S,), generator=g, device="cuda", dtype=torch.int32) for _ in range(2)]
+    off = [torch.tensor([0, S // 5, S // 2, S], dtype=torch.int32, device="cuda"), torch.tensor([0, 0, S - 1, S], dtype=torch.int32, device="cuda")]
+    bias = rand(g, E, N)
+    call = lambda x, i: call_grouped(ops, x, w, sa, sw, off[i], rows=rows[i], bias=bias, gelu=True)
+    want = [[call(x, i) for i in range(2)] for x in alt]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(4):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(call(alt[0], i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[0][i]) for o in got[i])
+    del got
+    x = alt[0].clone()
+    graphs, outs = [], []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            outs.append(call(x, i))
+    for j in (1, 0, 1):
+        x.copy_(alt[j])
+        for gr in graphs:
+            gr.replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(outs[i], want[j][i])
+    ops.check_status()
+
+
 @pytest.mark.parametrize("S", [4, 300])
 def test_gemm_grouped_tells_rows_and_columns_apart(ops, S):
     """One-hot operands: every output says which row, column and expert it came from."""
