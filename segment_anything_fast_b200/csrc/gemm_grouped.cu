@@ -211,8 +211,8 @@ grouped_one_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     const int tiles = tile_list(p, BM, s_first, s_start);
     if (lane == 0) {
       // Column tile: waves x what a tile takes, in columns a K step: its own, as much as 64 more for its rows, and some 1000
-      // in all for its start and epilogue.  A last wave that is mostly empty makes narrower tiles the better ones (3072
-      // rows of 16 experts, 1280 x 5120: 192 columns 70 us, 256 columns 87 us).
+      // in all for its start and epilogue.  A last wave that is mostly empty makes narrower tiles the better ones (2560
+      // rows of 16 experts, 1280 x 5120: 192 columns 65 us, 256 columns 73 us).
       long long best = 0;
       int bn = BN;
       for (int w = BN; w >= 64; w -= 64) {
