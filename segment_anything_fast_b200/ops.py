@@ -57,7 +57,7 @@ def _need(t: torch.Tensor, dtype: torch.dtype, name: str) -> None:
         raise RuntimeError(f"{name}: expected a CUDA tensor (there is no CPU path)")
     if t.dtype != dtype:
         raise RuntimeError(f"{name}: expected {dtype}, got {t.dtype}")
-    _same_device(t.get_device(), name)
+    _same_device(t.device.index, name)
 
 
 def _rows2d(t: torch.Tensor, name: str) -> torch.Tensor:
