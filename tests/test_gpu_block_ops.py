@@ -326,6 +326,22 @@ def test_route_strided_and_empty(ops):
     assert r.ids.shape == (0, 2) and r.rows.numel() == 0 and r.offsets.tolist() == [0] * 9
 
 
+@pytest.mark.parametrize("T,E,k", [(5, 16, 2), (300, 24, 3), (1000, 64, 8), (129, 60, 5), (200, 128, 4)])
+def test_route_whatever_the_alignment(ops, T, E, k):
+    """Rows that start off 16-byte boundaries, an odd pitch, a bias off its boundary: the same results."""
+    g = gen(T * E)
+    x, b = (2 * rand(g, T, E)).round(), rand(g, E).round()
+    want = ops.route_topk(x, k, bias=b)
+    check_route(ops, x, k, b)
+    flat = torch.zeros(T * (E + 9) + 1, device="cuda")
+    off_bias = torch.empty(E + 1, device="cuda")[1:].copy_(b)
+    for pitch, first in ((E + 8, 0), (E + 8, 1), (E + 9, 0), (E, 1)):
+        view = flat.as_strided((T, E), (pitch, 1), first).copy_(x)
+        for bias in (b, off_bias):
+            for p, q in zip(ops.route_topk(view, k, bias=bias), want):
+                assert torch.equal(p, q)
+
+
 # ------------------------------------------------------------------------------------------------ grouped products
 def grouped64(a, w, offsets, rows, bias, gelu, S, a_scale=None, w_scale=None):
     """Outputs, slack and which rows are written.  fp32 accumulation in the tensor core: K products, each addition off
