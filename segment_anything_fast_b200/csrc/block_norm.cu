@@ -394,16 +394,24 @@ block_norm_kernel(const NormParams p) {
   }
 }
 
+// Dynamic shared memory of block_norm_rows_kernel: two turns of four rows of h and r.
+constexpr int ring_bytes(int warps) { return 2 * 2 * 4 * warps * 32 * int(sizeof(uint4)); }
+constexpr int kStaticBytes = 2 * 2 * 32 * int(sizeof(float2)) + 32 * int(sizeof(float));
+static_assert(ring_bytes(5) + kStaticBytes <= 48 * 1024, "up to five warps need no opt-in");
+
 template <typename T, bool kRms, bool kQuant>
 int launch_typed(NormParams& p, cudaStream_t st) {
   const int warps = (p.C + 255) / 256, threads = warps * 32;
   const bool wide = warps > 8;
-  const int smem = 2 * 2 * 4 * threads * int(sizeof(uint4));
+  const int smem = ring_bytes(warps);
   auto rows4 = warps <= 5 ? block_norm_rows_kernel<T, kRms, kQuant, 5> : block_norm_rows_kernel<T, kRms, kQuant, 8>;
   static int cached_blocks[9] = {0};                     // resident blocks per SM by warps (a device fact, asked once)
   int blocks_sm = 0;
   if (!wide) {
-    if (smem > 48 * 1024 && cudaFuncSetAttribute(rows4, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    // Above the 48 KB that a kernel may use unasked, counting its static arrays too (six warps: 48 KB of ring alone).  Always
+    // the kernel's largest ring: the limit belongs to the kernel, and another host thread may be about to launch it.
+    if (warps > 5 &&
+        cudaFuncSetAttribute(rows4, cudaFuncAttributeMaxDynamicSharedMemorySize, ring_bytes(8)) != cudaSuccess)
       return SAMB_E_LAUNCH;
     int& n = cached_blocks[warps];
     if (n == 0) {
