@@ -201,7 +201,7 @@ block_norm_rows_kernel(const NormParams p) {
   const int threads = blockDim.x, c = int(threadIdx.x) * 8;
   const bool live = c < p.C;
   const int begin = int(blockIdx.x) * p.rows_per_block;
-  const int end = min(p.rows, begin + p.rows_per_block);
+  const int end = begin + min(p.rows_per_block, p.rows - begin);       // begin + rows_per_block may pass 2^31
   const bool has_post = p.post_g != nullptr, has_pre = p.pre_g != nullptr, has_res = p.r != nullptr;
   uint4* mine = ring + threadIdx.x;
   const uint16_t* h = static_cast<const uint16_t*>(p.h) + c;
@@ -322,7 +322,7 @@ block_norm_kernel(const NormParams p) {
   const int c = int(threadIdx.x) * 8;
   const bool live = c < p.C;
   const int begin = int(blockIdx.x) * p.rows_per_block;
-  const int end = min(p.rows, begin + p.rows_per_block);
+  const int end = begin + min(p.rows_per_block, p.rows - begin);       // begin + rows_per_block may pass 2^31
   const bool has_post = p.post_g != nullptr, has_pre = p.pre_g != nullptr;
 
   float pg[8], pb[8], qg[8], qb[8];          // post's gain and offset (times the gate), pre's gain and offset
@@ -425,12 +425,12 @@ int launch_typed(NormParams& p, cudaStream_t st) {
   const long long slots = (long long)sm_count() * blocks_sm;
   if (!wide && p.rows >= 4 * slots) {                    // four rows for every resident block: one resident wave
     p.rows_per_block = int(((p.rows + slots - 1) / slots + 3) / 4 * 4);
-    rows4<<<unsigned((p.rows + p.rows_per_block - 1) / p.rows_per_block), threads, smem, st>>>(p);
+    rows4<<<unsigned((p.rows - 1) / p.rows_per_block + 1), threads, smem, st>>>(p);
     return launch_status();
   }
   const long long most = (long long)sm_count() * (wide ? 2 : 8);
   p.rows_per_block = int((p.rows + most - 1) / most);
-  const unsigned blocks = unsigned((p.rows + p.rows_per_block - 1) / p.rows_per_block);
+  const unsigned blocks = unsigned((p.rows - 1) / p.rows_per_block + 1);
   if (wide) block_norm_kernel<T, kRms, kQuant, true><<<blocks, threads, 0, st>>>(p);
   else block_norm_kernel<T, kRms, kQuant, false><<<blocks, threads, 0, st>>>(p);
   return launch_status();

@@ -50,3 +50,14 @@ for t in (torch.bfloat16, torch.float16):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_block_norm_most_rows(ops):
+    """As many rows as the call takes: the last block's end is next to 2^31."""
+    rows, C = 0x7fffff00, 8
+    h = torch.ones(rows, C, dtype=BF16, device="cuda")
+    gate, pre = torch.full((C,), 2.0, device="cuda"), (torch.ones(C, device="cuda"), torch.full((C,), 3.0, device="cuda"))
+    x, y = ops.block_norm(h, gate=gate, pre=pre, out=h)
+    assert x.data_ptr() == h.data_ptr()
+    for lo in range(0, rows, 1 << 26):
+        assert (x[lo:lo + (1 << 26)] == 2).all() and (y[lo:lo + (1 << 26)] == 3).all(), lo
