@@ -13,8 +13,13 @@ from ._lib import EPI_BIAS, EPI_GELU, EPI_RAW, EPI_RESIDUAL  # noqa: F401  (re-e
 _status_words = {}
 
 
+# The current stream of a device, as a pointer; a torch built without CUDA lacks the short way, and imports this module too.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
 def _stream() -> int:
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return _raw_stream(torch.cuda.current_device())
 
 
 def _same_device(index: Optional[int], name: str) -> None:
@@ -543,9 +548,6 @@ def normalize_u8(x: torch.Tensor, mean, std, out: Optional[torch.Tensor] = None)
 # of experts.  16-bit tensors are bfloat16 or float16.
 # ---------------------------------------------------------------------------------------------------------------
 _F32, _F16, _BF16, _I32 = torch.float32, torch.float16, torch.bfloat16, torch.int32
-
-
-_raw_stream = torch._C._cuda_getCurrentRawStream       # the current stream of a device, as a pointer
 
 
 def _here(t: torch.Tensor, dtype: torch.dtype, dev: int, name: str) -> None:
