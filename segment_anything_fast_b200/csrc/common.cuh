@@ -379,23 +379,31 @@ __host__ __device__ constexpr uint32_t make_idesc(uint32_t acc_fmt, uint32_t a_f
          (uint32_t(b_mn_major) << 16) | (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
 }
 
-// Exact-form GELU x * Phi(x) = max(x, 0) - |x| * erfc(|x| / sqrt 2) / 2.  log2(erfc(a / sqrt 2) / 2) is smooth on
-// [0, 6.08] (beyond it the term is below 1e-9 |x|) and a degree-7 polynomial in a = |x| (Chebyshev fit) follows it
-// closely enough that the result is within 5.1e-7 of the exact GELU everywhere, far below the bf16 output rounding:
-// seven FMAs and one ex2, no division (the erf rational approximations cost a second special-function op, which is
-// what binds the int8 GEMM epilogue).
+// max(-|x|, -6.0811), and NaN where x is NaN
+__device__ __forceinline__ float gelu_clamp(float x) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(-fabsf(x)), "f"(-6.0811f));
+  return r;
+}
+
+// Exact-form GELU x * Phi(x) = max(x, 0) - a * erfc(a / sqrt 2) / 2, a = |x|.  log2(erfc(a / sqrt 2) / 2) is smooth on
+// [0, 6.08] and a degree-7 polynomial in a (Chebyshev fit) follows it closely enough that the result is within 5.1e-7 of the
+// exact GELU, far below the bf16 output rounding: seven FMAs and one ex2, no division (the erf rational approximations
+// cost a second special-function op, which is what binds the int8 GEMM epilogue).  Beyond 6.08 the whole term a * erfc stays
+// at its value there, 3.6e-9 (clamping erfc alone would leave 6e-10 |x|: -6 at x = -1e10 and inf - inf at +inf), so the
+// bound holds everywhere.  The polynomial runs in -a: the factor of the term and its argument are one register.
 __device__ __forceinline__ float gelu_erf(float x) {
-  const float a = fminf(fabsf(x), 6.0811f);
-  float q = fmaf(-1.926999857e-06f, a, 6.350679178e-05f);
-  q = fmaf(q, a, -9.461226873e-04f);
-  q = fmaf(q, a, 8.571726270e-03f);
-  q = fmaf(q, a, -5.409686640e-02f);
-  q = fmaf(q, a, -4.583186507e-01f);
-  q = fmaf(q, a, -1.151316047e+00f);
-  q = fmaf(q, a, -9.999877214e-01f);
+  const float na = gelu_clamp(x);
+  float q = fmaf(1.926999857e-06f, na, 6.350679178e-05f);
+  q = fmaf(q, na, 9.461226873e-04f);
+  q = fmaf(q, na, 8.571726270e-03f);
+  q = fmaf(q, na, 5.409686640e-02f);
+  q = fmaf(q, na, -4.583186507e-01f);
+  q = fmaf(q, na, 1.151316047e+00f);
+  q = fmaf(q, na, -9.999877214e-01f);
   float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(q));
-  return fmaf(-fabsf(x), e, fmaxf(x, 0.0f));
+  return fmaf(na, e, fmaxf(x, 0.0f));
 }
 
 // Packed fp32 pairs (sm_100: one instruction performs two IEEE fp32 operations on a 64-bit register pair; each
@@ -440,19 +448,19 @@ __device__ __forceinline__ f32x2 bf16x2_to_f32x2(uint32_t w) {
 __device__ __forceinline__ f32x2 gelu_erf2(f32x2 x2) {
   float x0, x1;
   unpack2(x2, x0, x1);
-  const f32x2 a2 = pack2(fminf(fabsf(x0), 6.0811f), fminf(fabsf(x1), 6.0811f));
-  f32x2 q = ffma2(pack2(-1.926999857e-06f, -1.926999857e-06f), a2, pack2(6.350679178e-05f, 6.350679178e-05f));
-  q = ffma2(q, a2, pack2(-9.461226873e-04f, -9.461226873e-04f));
-  q = ffma2(q, a2, pack2(8.571726270e-03f, 8.571726270e-03f));
-  q = ffma2(q, a2, pack2(-5.409686640e-02f, -5.409686640e-02f));
-  q = ffma2(q, a2, pack2(-4.583186507e-01f, -4.583186507e-01f));
-  q = ffma2(q, a2, pack2(-1.151316047e+00f, -1.151316047e+00f));
-  q = ffma2(q, a2, pack2(-9.999877214e-01f, -9.999877214e-01f));
+  const f32x2 na2 = pack2(gelu_clamp(x0), gelu_clamp(x1));
+  f32x2 q = ffma2(pack2(1.926999857e-06f, 1.926999857e-06f), na2, pack2(6.350679178e-05f, 6.350679178e-05f));
+  q = ffma2(q, na2, pack2(9.461226873e-04f, 9.461226873e-04f));
+  q = ffma2(q, na2, pack2(8.571726270e-03f, 8.571726270e-03f));
+  q = ffma2(q, na2, pack2(5.409686640e-02f, 5.409686640e-02f));
+  q = ffma2(q, na2, pack2(-4.583186507e-01f, -4.583186507e-01f));
+  q = ffma2(q, na2, pack2(1.151316047e+00f, 1.151316047e+00f));
+  q = ffma2(q, na2, pack2(-9.999877214e-01f, -9.999877214e-01f));
   float q0, q1, e0, e1;
   unpack2(q, q0, q1);
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(q0));
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(q1));
-  return ffma2(pack2(-fabsf(x0), -fabsf(x1)), pack2(e0, e1), pack2(fmaxf(x0, 0.0f), fmaxf(x1, 0.0f)));
+  return ffma2(na2, pack2(e0, e1), pack2(fmaxf(x0, 0.0f), fmaxf(x1, 0.0f)));
 }
 
 // Eight accumulator columns of one output row through the GEMM epilogue arithmetic, two at a time:

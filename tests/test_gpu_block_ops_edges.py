@@ -1,5 +1,6 @@
 """Block operators at widths, views, sizes and values that the calls accept and that are easily got wrong, against their
 formulas in 64 bits (bounds and helpers as in test_gpu_block_ops)."""
+import math
 import os
 import subprocess
 import sys
@@ -7,7 +8,7 @@ import sys
 import pytest
 import torch
 
-from test_gpu_block_ops import BF16, F16, block64, gen, near, ops, rand  # noqa: F401  (ops: fixture)
+from test_gpu_block_ops import BF16, F16, block64, call_grouped, gen, near, operands, ops, rand  # noqa: F401  (ops: fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -61,3 +62,57 @@ def test_block_norm_most_rows(ops):
     assert x.data_ptr() == h.data_ptr()
     for lo in range(0, rows, 1 << 26):
         assert (x[lo:lo + (1 << 26)] == 2).all() and (y[lo:lo + (1 << 26)] == 3).all(), lo
+
+
+# ------------------------------------------------------------------------------------------------ GELU over all numbers
+def gelu_values(N):
+    """Arguments from the middle to where fp32 ends, both signs, infinities and NaN in front."""
+    v = torch.cat([torch.logspace(-3, 38, N // 2 - 2), torch.tensor([6.08, 6.09])]).repeat_interleave(2)
+    v[1::2] *= -1
+    v[:3] = torch.tensor([math.inf, -math.inf, math.nan])
+    return v.cuda()
+
+
+def near_gelu(got, x):
+    """Within 5.1e-7 of the exact value and one rounding; infinities and NaN as they are."""
+    x = x.double()
+    want = torch.where(x == -math.inf, torch.zeros_like(x), x * torch.special.ndtr(x))
+    top = torch.finfo(got.dtype).max
+    over = want >= top * (1 + torch.finfo(got.dtype).eps / 4)        # rounds to infinity
+    assert (got[over & ~x.isnan()] == math.inf).all() and (got.isnan() == x.isnan()).all()
+    keep = want.abs() < top * 0.99
+    near(got[keep], want[keep], torch.full_like(want, 5.1e-7)[keep])
+
+
+@pytest.mark.parametrize("t", [BF16, F16, torch.int8])
+@pytest.mark.parametrize("S,E,N,K", [(3, 2, 136, 64), (300, 2, 136, 64), (17000, 3, 2568, 1024)])
+def test_grouped_gelu_over_all_numbers(ops, S, E, N, K, t):
+    """Warp dot products, single CTAs and CTA pairs: rows of zeros leave the bias as GELU's argument."""
+    g = gen(S)
+    a, w, sa, sw = operands(g, t, S, E, N, K)
+    a.zero_()
+    bias = gelu_values(N).expand(E, N).contiguous()
+    off = torch.tensor([0] + [S * (e + 1) // E for e in range(E)], dtype=torch.int32, device="cuda")
+    got = call_grouped(ops, a, w, sa, sw, off, bias=bias, gelu=True)
+    ops.check_status()
+    near_gelu(got, bias[:1].expand(S, N))
+
+
+def test_dense_gelu_over_all_numbers(ops):
+    N, K = 256, 64
+    bias = gelu_values(N)
+    w = torch.ones(N, K, dtype=BF16, device="cuda")
+    for M in (100, 20000):                               # single CTAs, CTA pairs
+        near_gelu(ops.gemm_bf16(torch.zeros(M, K, dtype=BF16, device="cuda"), w, bias, gelu=True), bias.expand(M, N))
+        near_gelu(ops.gemm_i8(torch.zeros(M, K, dtype=torch.int8, device="cuda"), torch.ones(M, device="cuda"), w.to(torch.int8),
+                              torch.ones(N, device="cuda"), bias, gelu=True), bias.expand(M, N))
+    wc, meta = ops.pack_sp24(torch.zeros(N, K, dtype=torch.int8, device="cuda"))
+    near_gelu(ops.gemm_i8_sp24(torch.zeros(300, K, dtype=torch.int8, device="cuda"), torch.ones(300, device="cuda"), wc, meta,
+                               torch.ones(N, device="cuda"), bias, gelu=True), bias.expand(300, N))
+    # quantised rows: a large negative argument leaves the row's largest value, GELU(1) = 0.84134 = 215.4 / 256, alone
+    for C in (1280, 5120):
+        x = torch.ones(33, C, dtype=BF16, device="cuda")
+        x[:, ::2] = -1e10
+        q, s = ops.quant_rows_i8(x, gelu=True)
+        assert torch.equal(s, torch.full_like(s, 215 / 256 / 127)) and (q[:, ::2] == 0).all() and (q[:, 1::2] == 127).all()
+    ops.check_status()
