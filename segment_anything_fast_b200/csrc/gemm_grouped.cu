@@ -53,13 +53,14 @@ struct GroupedParams {
   int k_bytes, k_slabs, last_ksteps;
 };
 
-// mbar_wait by a warp in step.  The lanes take the same decision without a vote on the way through: a phase that one lane
-// has seen complete stays so for the others, and where the wait gives up the lanes still there look once more
-// together.  (A vote after every wait of the MMA warp cost 4 to 7 % of a large product: 145 against 139 us at 16384 x 5120 x
-// 1280, and 163 us when one lane alone walks the loop.)
+// mbar_wait by a warp in step; each lane has its own answer.  A wait that runs out may run out for some lanes only (a
+// phase can complete between two lanes' last looks), and a lane that left its role alone would never come to the
+// elect.sync and __syncwarp that the others go on to.  So the lanes keep their answers for themselves: one that has given up
+// waits and issues no more (`ok` stays false), goes through the rest of the tile with its warp, and the warp
+// votes at the tile's end and leaves its role together.  (A vote after every wait of the MMA warp cost 4 to 7 % of a large
+// product: 145 against 139 us at 16384 x 5120 x 1280, and 163 us when one lane alone walks the loop.)
 __device__ __noinline__ bool warp_wait_long(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, uint32_t site) {
-  if (!mbar_wait(bar, parity, abort_flag, status, site)) return __any_sync(__activemask(), mbar_try_wait(bar, parity));
-  return true;
+  return mbar_wait(bar, parity, abort_flag, status, site);
 }
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, uint32_t site) {
   if (mbar_try_wait(bar, parity)) return true;
@@ -243,10 +244,10 @@ grouped_one_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       const int n0 = w.ntile * bn;
       const int a_boxes = w.rows > 2 * A_BOX_ROWS ? BM / A_BOX_ROWS : (w.rows + A_BOX_ROWS - 1) / A_BOX_ROWS;
       for (int ks = 0; ks < p.k_slabs; ++ks) {
-        if (!(ok = warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, 1))) break;
+        ok = ok && warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, 1);
         uint8_t* sa = smem + stage * STAGE_BYTES;
         uint64_t* bar = &full_bar[stage];
-        if (elect_one()) {
+        if (elect_one() && ok) {
           mbar_expect_tx(bar, (kGather ? (w.rows + 3) / 4 * 512 : a_boxes * A_BOX_BYTES) + bn * SLAB_BYTES);
           if (!kGather) {
             if (a_boxes == BM / A_BOX_ROWS) {
@@ -262,9 +263,10 @@ grouped_one_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
               tma_load_3d(sa + A_STAGE_BYTES + b * (64 * SLAB_BYTES), &tmB, bar, ks * slab_elems, n0 + b * 64, w.e);
         }
         __syncwarp();
-        ++issued;
+        if (ok) ++issued;
         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
       }
+      ok = __all_sync(0xffffffffu, ok);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issue
@@ -275,13 +277,13 @@ grouped_one_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
     bool ok = true;
     for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
-      if (!(ok = warp_wait(&acc_empty[acc], acc_phase ^ 1u, abort_flag, p.status, 2))) break;
+      ok = warp_wait(&acc_empty[acc], acc_phase ^ 1u, abort_flag, p.status, 2);
       tc_fence_after();
       const uint32_t d_tmem = tmem_base + acc * BN;
       for (int ks = 0; ks < p.k_slabs; ++ks) {
-        if (!(ok = warp_wait(&full_bar[stage], phase, abort_flag, p.status, 3))) break;
+        ok = ok && warp_wait(&full_bar[stage], phase, abort_flag, p.status, 3);
         tc_fence_after();
-        if (elect_one()) {
+        if (elect_one() && ok) {
           const uint64_t adesc = desc0 + stage * (STAGE_BYTES / 16);
           const uint64_t bdesc = adesc + A_STAGE_BYTES / 16;
           const int nsteps = ks == p.k_slabs - 1 ? p.last_ksteps : 4;
@@ -297,7 +299,7 @@ grouped_one_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         __syncwarp();
         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
       }
-      if (!ok) break;
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
       if (elect_one()) tc_commit(&acc_full[acc]);
       __syncwarp();
       if (++acc == NUM_ACC) { acc = 0; acc_phase ^= 1u; }
@@ -324,9 +326,9 @@ grouped_one_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 #pragma unroll
         for (int q = 0; q < 4; ++q) r[j][q] = __shfl_sync(0xffffffffu, mine[q], j);
       for (int ks = 0; ks < p.k_slabs; ++ks) {
-        if (!(ok = warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, 8))) break;
+        ok = ok && warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, 8);
         uint8_t* sa = smem + stage * STAGE_BYTES + g * 512;
-        if (elect_one()) {
+        if (elect_one() && ok) {
 #pragma unroll
           for (int j = 0; j < GATHER_GROUPS; ++j)
             if ((j * GATHER_WARPS + g) * 4 < w.rows)
@@ -336,6 +338,7 @@ grouped_one_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         __syncwarp();
         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
       }
+      ok = __all_sync(0xffffffffu, ok);
     }
   } else {
     // ------------------------------------------------------------------ epilogue
@@ -361,6 +364,7 @@ grouped_one_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         if (kInt8 && there) a_scale = __ldg(p.a_scale + i);
       }
       const bool got = mbar_wait(&acc_full[acc], acc_phase, abort_flag, p.status, 4);
+      __syncwarp();                                      // the barrier takes warps in step
       if (!epi_all(got)) break;                          // also publishes the column vectors
       tc_fence_after();
       const uint32_t t_addr = tmem_base + (lane_base << 16) + acc * BN + half * 32;
@@ -532,13 +536,13 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
       bool ok = true;
       for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
-        if (!(ok = warp_wait(&acc_empty[acc], acc_phase ^ 1u, abort_flag, p.status, 2))) break;
+        ok = warp_wait(&acc_empty[acc], acc_phase ^ 1u, abort_flag, p.status, 2);
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * BN;
         for (int ks = 0; ks < p.k_slabs; ++ks) {
-          if (!(ok = warp_wait(&full_bar[stage], phase, abort_flag, p.status, 3))) break;
+          ok = ok && warp_wait(&full_bar[stage], phase, abort_flag, p.status, 3);
           tc_fence_after();
-          if (elect_one()) {
+          if (elect_one() && ok) {
             const uint64_t adesc = desc0 + stage * (STAGE_BYTES / 16);
             const uint64_t bdesc = adesc + A_STAGE_BYTES / 16;
             const int nsteps = ks == p.k_slabs - 1 ? p.last_ksteps : 4;
@@ -555,7 +559,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           __syncwarp();
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
         }
-        if (!ok) break;
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
         if (elect_one()) {
           tc_commit_pair(accf_own + acc * 8);
           tc_commit_pair(accf_peer + acc * 8);
