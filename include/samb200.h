@@ -338,7 +338,8 @@ int samb_mask_rle(const uint8_t* masks, int64_t N, int H, int W, int32_t* counts
 /* ---------------------------------------------------------------------------------------------
  * Operators of transformer blocks beside the reference's own kind (no counterpart in the reference): norms around a
  * block, rotary positions, a mixture of experts.  16-bit tensors are bf16, or float16 when is_f16 != 0.  Outputs and
- * scratch share no memory with one another or with inputs, except where a comment says that one may be the other.
+ * scratch share no memory with one another or with inputs, except where a comment says that one may be the other; the norms,
+ * rotary positions, products and combination refuse a call that breaks this (SAMB_E_BADARG).
  * ------------------------------------------------------------------------------------------- */
 
 /* The norms before and after a residual addition, with the block's gate and the residual's scale:

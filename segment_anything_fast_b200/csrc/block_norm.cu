@@ -16,6 +16,7 @@
 // Bound by HBM: 235 us for 131072 x 1280 bf16 with both norms and a gate an image (1.34 GB, 5.7 TB/s); a row at a time through
 // registers took 635 us, held up by its barriers and shuffles.
 #include "elem16.cuh"
+#include "overlap.h"
 
 namespace samb {
 namespace {
@@ -455,6 +456,19 @@ int launch_block_norm(const void* h, int64_t ldh, const void* r, int64_t ldr, co
                         reinterpret_cast<uintptr_t>(pre_g) | reinterpret_cast<uintptr_t>(pre_b) |
                         reinterpret_cast<uintptr_t>(gate) | reinterpret_cast<uintptr_t>(y);
   if ((mis & 15u) || (reinterpret_cast<uintptr_t>(y_scale) & 3u)) return SAMB_E_ALIGN;
+  {
+    // what is written is memory of its own, or lies exactly over rows that the call may replace (checked above)
+    const Runs rh = rows_of(h, 2 * ldh, rows, 2 * C), rr = rows_of(r, 2 * ldr, rows, 2 * C), rx = rows_of(x, 2 * ldx, rows, 2 * C);
+    const Runs ry = bytes_of(y, rows * C * (quant ? 1 : 2)), rs = bytes_of(quant ? y_scale : nullptr, rows * 4);
+    const Runs vec[5] = {bytes_of(post_g, 4 * C), bytes_of(post_b, 4 * C), bytes_of(pre_g, 4 * C), bytes_of(pre_b, 4 * C),
+                         bytes_of(gate, 4 * gate_rows * C)};
+    if ((x != h && share_memory(rx, rh)) || (x != r && share_memory(rx, rr)) || (y != h && share_memory(ry, rh)) ||
+        (y != r && share_memory(ry, rr)) || share_memory(rx, ry) || share_memory(rs, rh) || share_memory(rs, rr) ||
+        share_memory(rs, rx) || share_memory(rs, ry))
+      return SAMB_E_BADARG;
+    for (const Runs& v : vec)
+      if (share_memory(v, rx) || share_memory(v, ry) || share_memory(v, rs)) return SAMB_E_BADARG;
+  }
   if (int e = check_device_arch()) return e;
   if (rows == 0) return SAMB_OK;
   NormParams p;

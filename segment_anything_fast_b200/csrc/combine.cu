@@ -3,6 +3,7 @@
 // nothing.  Bound by HBM: every row of x is read once; a thread owns eight columns of a token and has the loads of
 // all its choices in flight together.  51 us for 32768 tokens x 2 choices x 1280 bf16 with the residual (335 MB, 6.6 TB/s).
 #include "elem16.cuh"
+#include "overlap.h"
 
 namespace samb {
 namespace {
@@ -87,6 +88,13 @@ int samb_combine_topk(const void* x, int64_t ldx, int64_t x_rows, const int32_t*
   if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(residual) | reinterpret_cast<uintptr_t>(out)) & 15u)
     return SAMB_E_ALIGN;
   if ((reinterpret_cast<uintptr_t>(slots) | reinterpret_cast<uintptr_t>(weights)) & 3u) return SAMB_E_ALIGN;
+  {
+    const Runs ro = rows_of(out, 2 * ldo, T, 2 * C);
+    if (share_memory(ro, rows_of(x, 2 * ldx, x_rows, 2 * C)) || share_memory(ro, bytes_of(slots, 4 * T * k)) ||
+        share_memory(ro, bytes_of(weights, 4 * T * k)) ||
+        (out != residual && share_memory(ro, rows_of(residual, 2 * ldr, T, 2 * C))))
+      return SAMB_E_BADARG;
+  }
   if (int e = check_device_arch()) return e;
   if (T == 0) return SAMB_OK;
   CombineParams p;

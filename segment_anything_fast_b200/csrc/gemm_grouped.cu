@@ -23,6 +23,7 @@
 // row of the product depends on its own row of A alone), but stores only its own: whole tiles leave by TMA, the last
 // ones of an expert row by row.
 #include "elem16.cuh"
+#include "overlap.h"
 
 namespace samb {
 namespace {
@@ -983,6 +984,17 @@ int launch_grouped(int type, const void* A, int64_t lda, int64_t a_rows, const f
   if ((reinterpret_cast<uintptr_t>(rows) | reinterpret_cast<uintptr_t>(offsets) | reinterpret_cast<uintptr_t>(bias) |
        reinterpret_cast<uintptr_t>(a_scale) | reinterpret_cast<uintptr_t>(w_scale)) & 3u)
     return SAMB_E_ALIGN;
+  if (S > 0) {
+    const int64_t room = rows != nullptr && want_order(S, E, N, int64_t(K) * esz, type == kTypeI8) ? S * K * esz : 0;
+    const Runs written[2] = {rows_of(out, 2 * ldo, S, 2 * int64_t(N)), bytes_of(scratch, room)};
+    const Runs read[7] = {rows_of(A, lda * esz, a_rows, int64_t(K) * esz), runs3(W, w_stride * esz, E, ldw * esz, N, int64_t(K) * esz),
+                          bytes_of(bias, 4 * int64_t(E) * N), bytes_of(offsets, 4 * (int64_t(E) + 1)), bytes_of(rows, 4 * S),
+                          bytes_of(a_scale, 4 * a_rows), bytes_of(w_scale, 4 * int64_t(E) * N)};
+    if (share_memory(written[0], written[1])) return SAMB_E_BADARG;
+    for (const Runs& w : written)
+      for (const Runs& r : read)
+        if (share_memory(w, r)) return SAMB_E_BADARG;
+  }
   if (int e = check_device_arch()) return e;
   if (S == 0) return SAMB_OK;
 

@@ -14,6 +14,7 @@
 // positions), so the angles are worked out once and the copies stream, four of them in flight a thread.  Bound by HBM:
 // 57 us for 32 planes x 32768 rows x 80 bf16 (335 MB, 5.9 TB/s; 62 us with one copy in flight).
 #include "elem16.cuh"
+#include "overlap.h"
 
 namespace samb {
 namespace {
@@ -199,6 +200,13 @@ int samb_rotary(const void* x, int64_t plane_stride, int64_t row_stride, const v
     const int64_t n_outer = by_row ? rows : planes, n_inner = by_row ? planes : rows;
     if ((n_inner > 1 && inner < d) || (n_outer > 1 && outer < (n_inner > 1 ? (n_inner - 1) * inner : 0) + d))
       return SAMB_E_SHAPE;
+  }
+  {
+    const Runs ro = runs3(out, 2 * out_plane_stride, planes, 2 * out_row_stride, rows, 2 * d);
+    if ((x != out && share_memory(ro, runs3(x, 2 * plane_stride, planes, 2 * row_stride, rows, 2 * d))) ||
+        share_memory(ro, bytes_of(positions, rows > 0 ? period * axes * (positions_i64 ? 8 : 4) : 0)) ||
+        share_memory(ro, bytes_of(freqs, 4 * int64_t(rot))))
+      return SAMB_E_BADARG;
   }
   if (int e = check_device_arch()) return e;
   if (rows == 0 || planes == 0) return SAMB_OK;

@@ -546,6 +546,7 @@ def normalize_u8(x: torch.Tensor, mean, std, out: Optional[torch.Tensor] = None)
 # ---------------------------------------------------------------------------------------------------------------
 # Operators of transformer blocks beside the reference's own kind: norms around a block, rotary positions, a mixture
 # of experts.  16-bit tensors are bfloat16 or float16.
+# An ``out`` is memory of its own or the operand itself that the docstring allows; any other overlap is refused.
 # ---------------------------------------------------------------------------------------------------------------
 _F32, _F16, _BF16, _I32 = torch.float32, torch.float16, torch.bfloat16, torch.int32
 

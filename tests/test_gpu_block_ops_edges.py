@@ -116,3 +116,59 @@ def test_dense_gelu_over_all_numbers(ops):
         q, s = ops.quant_rows_i8(x, gelu=True)
         assert torch.equal(s, torch.full_like(s, 215 / 256 / 127)) and (q[:, ::2] == 0).all() and (q[:, 1::2] == 127).all()
     ops.check_status()
+
+
+# ------------------------------------------------------------------------------------------------ overlapping operands
+def test_overlapping_outputs_are_refused(ops):
+    g = gen(5)
+    buf = rand(g, 40, 64, t=BF16)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    fr, f = ops.rotary_freqs(64)[0], torch.ones(64, device="cuda")
+    slots, wt = torch.zeros(20, 2, dtype=torch.int32, device="cuda"), torch.ones(20, 2, device="cuda")
+    w, flat = rand(g, 2, 64, 64, t=BF16), buf.view(-1)
+    before = buf.clone()
+    for call in (lambda: ops.block_norm(buf[:20], out=buf[1:21]), lambda: ops.block_norm(rand(g, 20, 64, t=BF16), buf[:20], out=buf[19:39]),
+                 lambda: ops.block_norm_quant_i8(buf[:20], None, None, (f, None), out=buf[4:24]),
+                 lambda: ops.block_norm(buf[:20, :32], out=buf[:20, 24:56]),
+                 lambda: ops.rotary(buf[None, :20], i32(0), fr, out=buf[None, 3:23]),
+                 lambda: ops.rotary(flat.as_strided((2, 10, 64), (640, 64, 1)), i32(0), fr, out=flat.as_strided((2, 10, 64), (64, 128, 1))),
+                 lambda: ops.gemm_grouped(buf[:20], w, i32(0, 10, 20), out=buf[19:39]),
+                 lambda: ops.gemm_grouped(rand(g, 20, 64, t=BF16), w, i32(0, 10, 20), out=w.view(128, 64)[100:120]),
+                 lambda: ops.combine_topk(buf[:20], slots, wt, out=buf[19:39]),
+                 lambda: ops.combine_topk(rand(g, 20, 64, t=BF16), slots, wt, residual=buf[:20], out=buf[1:21])):
+        with pytest.raises(RuntimeError, match="bad argument"):
+            call()
+    assert torch.equal(buf, before)
+
+
+def test_outputs_between_the_operands_rows(ops):
+    """Views of one buffer that share no element are as good as separate tensors."""
+    g = gen(6)
+    S, C = 300, 64
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    buf = rand(g, S, 5 * C, t=BF16)
+    a, b, out = buf[:, :C], buf[:, C:2 * C], buf[:, 3 * C:4 * C]
+    rest = buf.clone()
+    want, _ = ops.block_norm(a.contiguous(), b.contiguous())
+    ops.block_norm(a, b, out=out)
+    assert torch.equal(out, want)
+    w, off = rand(g, 2, C, C, t=BF16), i32(0, 100, S)
+    want = ops.gemm_grouped(a.contiguous(), w, off)
+    ops.gemm_grouped(a, w, off, out=out)
+    assert torch.equal(out, want)
+    slots, wt = torch.randint(-1, S, (S, 2), generator=g, device="cuda", dtype=torch.int32), rand(g, S, 2)
+    want = ops.combine_topk(a.contiguous(), slots, wt, residual=b.contiguous())
+    ops.combine_topk(a, slots, wt, residual=b, out=out)
+    assert torch.equal(out, want)
+    heads = lambda n: buf.as_strided((2, S, 32), (32, 5 * C, 1), n * C)
+    fr, _ = ops.rotary_freqs(32)
+    want = ops.rotary(heads(0).contiguous(), torch.arange(S, device="cuda"), fr)
+    ops.rotary(heads(0), torch.arange(S, device="cuda"), fr, out=heads(3))
+    assert torch.equal(heads(3), want)
+    rest[:, 3 * C:4 * C] = buf[:, 3 * C:4 * C]
+    assert torch.equal(buf, rest)
+    # rows of unlike pitch, one tensor between the other's rows
+    full = rand(g, 2, 10, C, t=BF16)
+    want, _ = ops.block_norm(full[:, 0].contiguous())
+    ops.block_norm(full[:, 0], out=full[0, 3:5])
+    assert torch.equal(full[0, 3:5], want)
