@@ -720,7 +720,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, interl
     ``qkv[:2 * H]`` of ``gemm_heads``, or a ``[rows, heads, d]`` tensor seen as ``x.transpose(0, 1)``).  Pairs are
     neighbours (``interleaved``) or half the rotated width apart; the first ``2 * len(freqs)`` elements of a row turn,
     the rest is copied.  ``positions`` int32 / int64: ``[P]``, or ``[P, 2]`` for a raster (first half of the pairs by the
-    first coordinate); row r uses entry ``r % P``.  ``freqs`` float64, see ``rotary_freqs``.  ``out`` may be ``x``."""
+    first coordinate); row r uses entry ``r % P``.  ``freqs`` float64, see ``rotary_freqs``.  ``out`` may be ``x``;
+    a new result has the order of x's axes, and rows padded to a multiple of 8 where d is none."""
     dtype, dev = _half(x, "x")
     _here(freqs, torch.float64, dev, "freqs")
     pt = positions.dtype
@@ -740,7 +741,12 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, interl
     if freqs.dim() != 1 or not freqs.is_contiguous():
         raise RuntimeError("freqs: expected a contiguous 1-D tensor")
     if out is None:
-        out = torch.empty_like(x)                         # laid out like x where x has no gaps
+        if d % 8 == 0:
+            out = torch.empty_like(x)                     # laid out like x where x has no gaps
+        elif ps < rs:                                     # rows start at multiples of 8, as those of x
+            out = torch.empty(rows, planes, -(-d // 8) * 8, dtype=dtype, device=x.device)[..., :d].transpose(0, 1)
+        else:
+            out = torch.empty(planes, rows, -(-d // 8) * 8, dtype=dtype, device=x.device)[..., :d]
     else:
         _here(out, dtype, dev, "out")
         if out.shape != x.shape:

@@ -8,7 +8,7 @@ import sys
 import pytest
 import torch
 
-from test_gpu_block_ops import BF16, F16, block64, call_grouped, gen, near, operands, ops, rand  # noqa: F401  (ops: fixture)
+from test_gpu_block_ops import BF16, F16, block64, call_grouped, gen, near, operands, ops, rand, rotary64  # noqa: F401  (ops: fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -172,3 +172,23 @@ def test_outputs_between_the_operands_rows(ops):
     want, _ = ops.block_norm(full[:, 0].contiguous())
     ops.block_norm(full[:, 0], out=full[0, 3:5])
     assert torch.equal(full[0, 3:5], want)
+
+
+# ------------------------------------------------------------------------------------------------ rotary widths
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("d,rot", [(20, 20), (20, 8), (2, 2), (30, 16), (12, 12), (81, 40)])
+def test_rotary_of_padded_rows(ops, d, rot, interleaved):
+    """Widths that are no multiples of 8, in rows that start at multiples of 8: the result is laid out alike."""
+    g = gen(d)
+    pad = -(-d // 8) * 8 + 8
+    pos = torch.randint(0, 5000, (35,), generator=g, device="cuda")
+    freqs, _ = ops.rotary_freqs(rot)
+    for x in (rand(g, 3, 70, pad, t=BF16)[..., :d], rand(g, 70, 3, pad, t=F16)[..., :d].transpose(0, 1)):
+        got = ops.rotary(x, pos, freqs, interleaved=interleaved)
+        assert got.shape == x.shape and (got.stride(0) < got.stride(1)) == (x.stride(0) < x.stride(1))
+        want, slack = rotary64(x, pos, freqs, interleaved, 1.0)
+        near(got, want, slack)
+        assert torch.equal(got[..., rot:], x[..., rot:])
+        own = rand(g, 3, 70, pad, t=x.dtype)
+        ops.rotary(x, pos, freqs, interleaved=interleaved, out=own[..., :d])
+        assert torch.equal(own[..., :d], got)
