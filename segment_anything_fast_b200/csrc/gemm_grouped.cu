@@ -1014,14 +1014,6 @@ int launch_grouped(int type, const void* A, int64_t lda, int64_t a_rows, const f
     const uint32_t box[3] = {slab_elems, uint32_t(box_rows), 1};
     return make_tensor_map(&tmB, dt, 3, const_cast<void*>(W), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
   };
-  {
-    const uint64_t dims[2] = {uint64_t(N), uint64_t(S)};
-    const uint64_t strides[2] = {2, uint64_t(ldo) * 2};
-    const uint32_t box[2] = {64, uint32_t(BM)};
-    if (int e = make_tensor_map(&tmOut, type == kTypeF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                                2, out, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
-      return e;
-  }
   GroupedParams p;
   p.out = out; p.a = static_cast<const uint8_t*>(A); p.bias = bias; p.a_scale = a_scale; p.w_scale = w_scale; p.rows = rows;
   p.offsets = offsets; p.status = status;
@@ -1038,6 +1030,14 @@ int launch_grouped(int type, const void* A, int64_t lda, int64_t a_rows, const f
     else if (type == kTypeF16) launch_few<kTypeF16>(w, pitch, stride, p, gelu, st);
     else launch_few<kTypeI8>(w, pitch, stride, p, gelu, st);
     return launch_status();
+  }
+  {
+    const uint64_t dims[2] = {uint64_t(N), uint64_t(S)};
+    const uint64_t strides[2] = {2, uint64_t(ldo) * 2};
+    const uint32_t box[2] = {64, uint32_t(BM)};
+    if (int e = make_tensor_map(&tmOut, type == kTypeF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                                2, out, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
+      return e;
   }
   // what the products read: A itself, or its rows in order in the caller's scratch
   const bool int8 = type == kTypeI8;

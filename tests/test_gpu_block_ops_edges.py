@@ -192,3 +192,17 @@ def test_rotary_of_padded_rows(ops, d, rot, interleaved):
         own = rand(g, 3, 70, pad, t=x.dtype)
         ops.rotary(x, pos, freqs, interleaved=interleaved, out=own[..., :d])
         assert torch.equal(own[..., :d], got)
+
+
+# ------------------------------------------------------------------------------------------------ few rows
+def test_grouped_few_rows_have_no_tensor_maps(ops):
+    """Up to eight rows are dot products: pitches that no tensor map takes (single rows, so nothing lies that far) are fine."""
+    from segment_anything_fast_b200 import _lib
+    g = gen(9)
+    a, w, off = rand(g, 1, 64, t=BF16), rand(g, 2, 32, 64, t=BF16), torch.tensor([0, 0, 1], dtype=torch.int32, device="cuda")
+    out = torch.zeros(1, 32, dtype=BF16, device="cuda")
+    rc = _lib.load().samb_gemm_grouped(a.data_ptr(), 1 << 40, 1, None, w.data_ptr(), 64, 64 * 32, None, off.data_ptr(), out.data_ptr(),
+                                       1 << 40, 1, 2, 32, 64, 0, 0, None, ops.status_word(a.device).data_ptr(),
+                                       torch.cuda.current_stream().cuda_stream)
+    assert rc == 0 and torch.equal(out, ops.gemm_grouped(a, w, off))
+    ops.check_status()
