@@ -15,6 +15,8 @@
 // sums share their shuffles: halves of the warp trade rows first, 6 shuffles instead of 20.
 // Bound by HBM: 235 us for 131072 x 1280 bf16 with both norms and a gate an image (1.34 GB, 5.7 TB/s); a row at a time through
 // registers took 635 us, held up by its barriers and shuffles.
+#include <atomic>
+
 #include "elem16.cuh"
 #include "overlap.h"
 
@@ -406,7 +408,8 @@ int launch_typed(NormParams& p, cudaStream_t st) {
   const bool wide = warps > 8;
   const int smem = ring_bytes(warps);
   auto rows4 = warps <= 5 ? block_norm_rows_kernel<T, kRms, kQuant, 5> : block_norm_rows_kernel<T, kRms, kQuant, 8>;
-  static int cached_blocks[9] = {0};                     // resident blocks per SM by warps (a device fact, asked once)
+  // resident blocks per SM by warps (a device fact, asked once; host threads may ask at once, and give the same answer)
+  static std::atomic<int> cached_blocks[9] = {};
   int blocks_sm = 0;
   if (!wide) {
     // Above the 48 KB that a kernel may use unasked, counting its static arrays too (six warps: 48 KB of ring alone).  Always
@@ -414,14 +417,12 @@ int launch_typed(NormParams& p, cudaStream_t st) {
     if (warps > 5 &&
         cudaFuncSetAttribute(rows4, cudaFuncAttributeMaxDynamicSharedMemorySize, ring_bytes(8)) != cudaSuccess)
       return SAMB_E_LAUNCH;
-    int& n = cached_blocks[warps];
-    if (n == 0) {
-      int got = 0;
-      if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&got, rows4, threads, size_t(smem)) != cudaSuccess || got < 1)
+    blocks_sm = cached_blocks[warps].load(std::memory_order_relaxed);
+    if (blocks_sm == 0) {
+      if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks_sm, rows4, threads, size_t(smem)) != cudaSuccess || blocks_sm < 1)
         return SAMB_E_LAUNCH;
-      n = got;
+      cached_blocks[warps].store(blocks_sm, std::memory_order_relaxed);
     }
-    blocks_sm = n;
   }
   const long long slots = (long long)sm_count() * blocks_sm;
   if (!wide && p.rows >= 4 * slots) {                    // four rows for every resident block: one resident wave

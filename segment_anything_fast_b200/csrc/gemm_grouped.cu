@@ -22,6 +22,8 @@
 // A tile computes all its rows whatever its expert has left (the rows behind them in shared memory may be anything: a
 // row of the product depends on its own row of A alone), but stores only its own: whole tiles leave by TMA, the last
 // ones of an expert row by row.
+#include <atomic>
+
 #include "elem16.cuh"
 #include "overlap.h"
 
@@ -942,12 +944,16 @@ int launch_pairs(int type, bool gelu, const CUtensorMap& tmA, const CUtensorMap&
   cfg.dynamicSmemBytes = size_t(smem_bytes);
   cfg.stream = st;
   cfg.gridDim = dim3(unsigned(sm_count() & ~1));
-  static int cached_clusters[3][4] = {};                  // co-resident pairs per kernel variant (0 = not asked yet)
-  int& max_clusters = cached_clusters[type][(bias ? 2 : 0) + (gelu ? 1 : 0)];
-  if (max_clusters == 0 &&
-      (cudaOccupancyMaxActiveClusters(&max_clusters, kern, &cfg) != cudaSuccess || max_clusters < 1)) {
-    cudaGetLastError();
-    max_clusters = -1;
+  // co-resident pairs per kernel variant (0 = not asked yet); host threads may ask at once, and give the same answer
+  static std::atomic<int> cached_clusters[3][4] = {};
+  std::atomic<int>& cached = cached_clusters[type][(bias ? 2 : 0) + (gelu ? 1 : 0)];
+  int max_clusters = cached.load(std::memory_order_relaxed);
+  if (max_clusters == 0) {
+    if (cudaOccupancyMaxActiveClusters(&max_clusters, kern, &cfg) != cudaSuccess || max_clusters < 1) {
+      cudaGetLastError();
+      max_clusters = -1;
+    }
+    cached.store(max_clusters, std::memory_order_relaxed);
   }
   if (max_clusters < 1) return SAMB_E_SHAPE;
   long long pairs = max_clusters < sm_count() / 2 ? max_clusters : sm_count() / 2;

@@ -206,3 +206,39 @@ def test_grouped_few_rows_have_no_tensor_maps(ops):
                                        torch.cuda.current_stream().cuda_stream)
     assert rc == 0 and torch.equal(out, ops.gemm_grouped(a, w, off))
     ops.check_status()
+
+
+# ------------------------------------------------------------------------------------------------ host threads
+def test_first_calls_from_several_threads(ops):
+    """ctypes lets go of the interpreter's lock: twelve threads make their first calls at once, each on its own stream."""
+    code = """
+import threading
+import torch
+from segment_anything_fast_b200 import ops
+torch.manual_seed(0)
+norms = [(torch.randn(5000, C, device="cuda").bfloat16(), torch.ones(C, device="cuda")) for C in (1280, 1536, 1792, 2048)]
+a, w = torch.randn(17000, 512, device="cuda").bfloat16(), torch.randn(3, 2568, 512, device="cuda").bfloat16()
+off = torch.tensor([0, 4000, 12000, 17000], dtype=torch.int32, device="cuda")
+rows = torch.randperm(17000, device="cuda", dtype=torch.int32)
+ops.status_word(a.device)
+calls = [lambda h=h, f=f: ops.block_norm(h, h, pre=(f, None))[1] for h, f in norms] * 2
+calls += [lambda: ops.gemm_grouped(a, w, off), lambda: ops.gemm_grouped(a, w, off, rows=rows)] * 2
+got, gate = [None] * len(calls), threading.Barrier(len(calls))
+streams = [torch.cuda.Stream() for _ in calls]
+torch.cuda.synchronize()
+def work(i):
+    with torch.cuda.stream(streams[i]):
+        gate.wait()
+        got[i] = [calls[i]() for _ in range(5)]
+threads = [threading.Thread(target=work, args=(i,)) for i in range(len(calls))]
+for t in threads: t.start()
+for t in threads: t.join()
+torch.cuda.synchronize()
+ops.check_status()
+for i, c in enumerate(calls):
+    want = c()
+    assert got[i] is not None and all(torch.equal(o, want) for o in got[i]), i
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
