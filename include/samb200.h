@@ -369,7 +369,7 @@ int samb_block_norm_quant_i8(const void* h, int64_t ldh, const void* residual, i
  * on are copied.  positions[period][axes] is int32, or int64 when positions_i64 != 0: row r uses entry r % period
  * (rows % period == 0).  With axes == 2 (rot % 4 == 0) the first half of the pairs turns with the first coordinate and
  * the second half with the second.  freqs: DEVICE array of rot / 2 doubles, radians a position.  The angle
- * is off by at most (2^-32 + |position| * 2^-63) turns.  out may be x itself with the same strides (in place). */
+ * is off by at most (2^-26 + 2^-32 + |position| * 2^-63) turns, the first for its rounding to fp32.  out may be x itself with the same strides (in place). */
 int samb_rotary(const void* x, int64_t plane_stride, int64_t row_stride, const void* positions, int positions_i64,
                 int64_t period, int axes, const double* freqs, int rot, int interleaved, float mscale, void* out,
                 int64_t out_plane_stride, int64_t out_row_stride, int64_t planes, int64_t rows, int d, int is_f16,

@@ -8,7 +8,9 @@
 // Angles: a float angle of position 10^6 is off by 0.06 rad, and reducing a double angle costs more than the
 // rotation.  A frequency is instead held as a 64-bit fixed-point fraction of a turn, F = frac(freq / 2 pi) * 2^64, and
 // position * F modulo 2^64 is the exact fraction of the turn that this F reaches: one integer product, no reduction.
-// Its top 32 bits are the argument of sincospi: the angle is off by 2^-32 turns and position * 2^-64 turns.
+// Its top 32 bits, rounded to fp32, are the argument of sincospi: the angle is off by at most 2^-32 turns (bits dropped), 2^-26
+// turns (fp32 holds 24 bits of up to half a turn; less for smaller angles) and position * 2^-63 turns (F: its own last
+// place, and the second part of the product that makes it).
 //
 // A thread owns V pairs of a position and walks over the copies that share it (planes x repetitions of the
 // positions), so the angles are worked out once and the copies stream, four of them in flight a thread.  Bound by HBM:

@@ -1,9 +1,11 @@
 """Block operators without a GPU: what the package needs of torch, and calls that are refused before a launch."""
+import math
 import os
 import random
 import re
 import subprocess
 import sys
+from fractions import Fraction
 
 import numpy as np
 import pytest
@@ -150,3 +152,26 @@ def test_outputs_over_small_operands_are_refused(lib):
     lib_rows = lambda scr: lib.samb_gemm_grouped(MB, 1280, 100, big["rows"], big["w"], 1280, 1280 * 5120, big["bias"], FAR, big["out"], 5120,
                                                  65536, 4, 5120, 1280, 0, 1, scr, FAR, None)
     assert lib_rows(1 << 39) != BAD and lib_rows(big["out"] + 1600) == BAD and lib_rows(MB) == BAD and lib_rows(big["rows"] - 16) == BAD
+
+
+def test_rotary_angle_keeps_the_bound_in_the_header():
+    """The kernel's arithmetic for an angle (64-bit fixed point, top 32 bits, fp32), restated, against whole numbers."""
+    text = open(os.path.join(ROOT, "include", "samb200.h")).read()
+    bound = re.search(r"off by at most \(([^)]*)\) turns", text).group(1).replace("^", "**").replace("|position|", "Fraction(pos)")
+    two_pi = Fraction(2 * 3141592653589793238462643383279502884197169399375105820974944592307816406286, 10 ** 75)
+    inv, inv_low, one = 0.15915494309189535, -9.839338337591243e-18, 2.0 ** 64
+    rng = random.Random(2)
+    worst = 0.0
+    for _ in range(5000):
+        f, pos = math.exp(rng.uniform(-14.0, 1.5)), rng.randint(0, 1 << rng.choice([6, 20, 40]))
+        hi = f * inv
+        lo = float(Fraction(f) * Fraction(inv) - Fraction(hi)) + f * inv_low
+        step = (int((hi - math.floor(hi)) * one) + int(lo * one)) % (1 << 64)
+        turn = (pos * step % (1 << 64)) >> 32
+        got = Fraction(float(np.float32(turn - (1 << 32) if turn >= 1 << 31 else turn))) / (1 << 32)
+        err = (got - Fraction(f) / two_pi * pos) % 1
+        err = min(err, 1 - err)
+        allowed = eval(bound, {"Fraction": Fraction, "pos": pos})
+        assert err <= allowed
+        worst = max(worst, float(err / allowed))
+    assert worst > 0.5                                   # and it says no more than it has to
