@@ -138,7 +138,8 @@ __device__ __forceinline__ void tma_gather4(void* smem_dst, const CUtensorMap* m
 }
 
 // A wait gave up somewhere: the producer sees its copies in flight home before the CTA ends.  Those whose barrier will
-// not complete any more (a partner stopped in between) get a tenth of a millisecond, many times what a copy takes.
+// not complete any more (a partner stopped in between), and products that were issued before their warp's vote, get a tenth of
+// a millisecond, many times what either takes; only then does the tensor memory go back.
 template <int STAGES>
 __device__ __forceinline__ void drain_copies(uint64_t* full_bar, uint32_t issued) {
   for (uint32_t i = issued > STAGES ? issued - STAGES : 0u; i < issued; ++i)
@@ -422,7 +423,10 @@ grouped_one_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 0 && *abort_flag) drain_copies<STAGES>(full_bar, issued);
+  if (*abort_flag) {                                     // the same for every thread: all roles have ended
+    if (warp == 0) drain_copies<STAGES>(full_bar, issued);
+    __syncthreads();
+  }
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, TMEM_COLS);

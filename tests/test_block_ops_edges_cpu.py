@@ -175,3 +175,11 @@ def test_rotary_angle_keeps_the_bound_in_the_header():
         assert err <= allowed
         worst = max(worst, float(err / allowed))
     assert worst > 0.5                                   # and it says no more than it has to
+
+
+def test_grouped_tensor_memory_goes_back_after_the_drain():
+    """A kernel that gave up waits for its copies and products in flight before it returns tensor memory: between the
+    drain by one warp and the release by another stands a barrier."""
+    text = re.sub(r"//[^\n]*", "", open(os.path.join(ROOT, "segment_anything_fast_b200", "csrc", "gemm_grouped.cu")).read())
+    ends = re.findall(r"drain_copies<STAGES>\(full_bar(.*?)tmem_dealloc", text, flags=re.S)
+    assert len(ends) == 2 and all("__syncthreads()" in e or "cluster_sync_all()" in e for e in ends)
