@@ -860,9 +860,13 @@ void launch_few(const uint8_t* W, long long w_pitch, long long w_stride, const G
   else grouped_few_kernel<kType, 1><<<grid, 32 * FEW_WARPS, 0, st>>>(W, w_pitch, w_stride, p, gelu);
 }
 
-// Rows in all up to which the dot products win.  16 experts, us, against the tile kernel: 5120 x 1280 bf16 15 / 19 at 8 rows,
-// 35 / 45 at 12, 34 / 43 at 16, 53 / 36 at 24; 1280 x 5120: 18 / 57 at 8, 38 / 59 at 12, 59 / 33 at 16; int8 5120 x 1280: 11 / 12 at 8,
-// 12 / 21 at 12, 18 / 19 at 16.
+// Rows in all up to which a call goes to the dot products.  us on the device with the weights in HBM, dot products / tile kernel,
+// rows spread over the experts | all with one.  16 experts, 5120 x 1280 bf16: 1 row 6.9 / 11.2; 2 rows 10.2 / 12.3 | 9.2 / 11.3;
+// 4 rows 18.5 / 16.1 | 11.8 / 11.2; 8 rows 24.9 / 19.3 | 18.4 / 11.5.  1280 x 5120 bf16: 2 rows 9.9 / 23.8 | 13.8 / 23.6; 4 rows
+// 14.3 / 29.5 | 22.3 / 23.4; 8 rows 30.6 / 30.4 | 49.8 / 23.6; 12 rows 41.9 / 34.2 | 72 / 23.5.  int8 5120 x 1280: 4 rows 10.7 / 11.8 |
+// 7.1 / 7.7; 8 rows 15.8 / 14.7 | 10.8 / 8.0; 12 rows 20.5 / 17.1 | 14.2 / 7.6.  32 experts, 512 x 512 bf16: 8 rows 4.1 / 8.0 |
+// 6.2 / 6.6; 12 rows 4.5 / 8.1 | 9.0 / 6.6.  The host does not know how the rows are spread: at eight the two sides are even over
+// these, above it the tile kernel is ahead but for small experts.
 constexpr int64_t kFewSlots = 8;
 
 // Rows of A in the order of the slots, packed: 16-byte vectors, several loads a thread in flight.  A row that does not
