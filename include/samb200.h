@@ -376,7 +376,8 @@ int samb_rotary(const void* x, int64_t plane_stride, int64_t row_stride, const v
                 void* stream);
 
 /* The router of a mixture of experts over logits[T, E] (fp32, leading dimension ld; E <= 512, k <= 8, k <= E):
- *   ids[T, k]      experts of the k largest logits (+ bias[e], when given: it decides the choice only), largest first,
+ *   ids[T, k]      experts of the k largest logits (+ bias[e], when given: it decides the choice only, and is added to the
+ *                  logit, not to its softmax or sigmoid, which would order experts differently), largest first,
  *                  ties to the lower index; -inf and NaN are never chosen, -1 stands where nobody is left
  *   weights[T, k]  softmax over the row's logits (or their sigmoid when sigmoid != 0) at the chosen experts, divided
  *                  by their sum when renorm != 0, times scale; 0 where ids is -1.  +inf counts as the largest float.
@@ -396,7 +397,7 @@ int samb_route_topk(const float* logits, int64_t ld, const float* bias, int64_t 
  * 16-byte aligned rows, N and K multiples of 8, E <= 512.  offsets[E + 1] is read on the device: values outside [0, S]
  * are clamped, and an expert whose range falls back behind an earlier one's is empty.  Rows of out outside every range
  * are left as they were.  rows (may be null; then a_rows >= S): an index outside [0, a_rows) stands for a row of
- * zeros.  epilogue: SAMB_EPI_BIAS (bias fp32 [E, N]) and / or SAMB_EPI_GELU.
+ * zeros; a_rows >= 1 where S is.  epilogue: SAMB_EPI_BIAS (bias fp32 [E, N]) and / or SAMB_EPI_GELU.
  * scratch: samb_gemm_grouped_scratch_bytes bytes (0 but for large products), 16-byte aligned, any contents, used with
  * rows only: large products put the rows in order there first.  Null is allowed and slower.  Calls that may overlap on the GPU
  * need one each. */

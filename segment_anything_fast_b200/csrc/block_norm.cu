@@ -13,8 +13,11 @@
 //   M2 = sum_w M2_w + n_w (mean_w - mean)^2,
 // so a norm costs one block barrier for four rows and no difference of large squares is ever taken.  The four rows'
 // sums share their shuffles: halves of the warp trade rows first, 6 shuffles instead of 20.
-// Bound by HBM: 235 us for 131072 x 1280 bf16 with both norms and a gate an image (1.34 GB, 5.7 TB/s); a row at a time through
-// registers took 635 us, held up by its barriers and shuffles.
+// Bound by HBM: 232 us for 131072 x 1280 bf16 with both norms and a gate an image (1.34 GB, 5.8 TB/s), 311 us for 1536 columns; a row at
+// a time through registers took 635 us, held up by its barriers and shuffles.  Above 2048 columns that is still the way: 298 us for
+// 16384 x 4096 (1.8 TB/s), 831 us for 16384 x 8192.  The quantised form is bound by instruction issue and the latency
+// behind it (63 % of the issue slots with 4.6 warps a scheduler, DRAM 29 %): 389 us for 131072 x 1280, where the 16-bit form and a
+// pass of samb_quant_rows_i8 take 346 us; 339 against 348 us for 16384 x 4096.
 #include <atomic>
 
 #include "elem16.cuh"

@@ -1,7 +1,7 @@
 // Combination of the experts' rows: y[t] = residual[t] + sum_j weights[t, j] * x[slots[t, j]], summed in fp32 in the
 // order of j and rounded once.  A slot outside x (the router gives -1 to a choice that a token did not make) adds
 // nothing.  Bound by HBM: every row of x is read once; a thread owns eight columns of a token and has the loads of
-// all its choices in flight together.  51 us for 32768 tokens x 2 choices x 1280 bf16 with the residual (335 MB, 6.6 TB/s).
+// all its choices in flight together.  52 us for 32768 tokens x 2 choices x 1280 bf16 with the residual (335 MB, 6.4 TB/s).
 #include "elem16.cuh"
 #include "overlap.h"
 

@@ -15,9 +15,10 @@
 // in caller scratch, is the better one (16384 x 5120 x 1280: 162 us against 160 us, but 127 against 135 us in int8, and 752
 // against 764 us at 65536 rows under the power cap).
 //
-// Measured, one B200: 65536 x 5120 x 1280 bf16 with 16 experts, gathered, bias and GELU: 650 us = 1.32 PFLOP/s (one dense
-// product of that size: 578 us here, 587 us by the vendor library); 16384 x 5120 x 1280 int8: 111 us = 1.9 POP/s; 2062 x 1280 x
-// 5120 f16: 48 us, 4.9 TB/s; one token with two experts of 5120 x 1280: 8.8 us, 3.0 TB/s.
+// Measured, one B200: 65536 x 5120 x 1280 bf16 with 16 experts, gathered, bias and GELU: 640 us = 1.34 PFLOP/s (one dense
+// product of that size: 578 us here, 587 us by the vendor library); 16384 x 5120 x 1280 int8: 111 us = 1.9 POP/s (rows in order 102, even
+// experts 96, one dense product 91); 2062 x 1280 x 5120 f16: 48 us, 4.9 TB/s; one token with two experts of 5120 x 1280, weights in
+// HBM: 10.2 us, 2.6 TB/s (13.2 us gathered with bias and GELU).
 //
 // A tile computes all its rows whatever its expert has left (the rows behind them in shared memory may be anything: a
 // row of the product depends on its own row of A alone), but stores only its own: whole tiles leave by TMA, the last

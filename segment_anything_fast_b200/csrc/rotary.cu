@@ -14,7 +14,7 @@
 //
 // A thread owns V pairs of a position and walks over the copies that share it (planes x repetitions of the
 // positions), so the angles are worked out once and the copies stream, four of them in flight a thread.  Bound by HBM:
-// 57 us for 32 planes x 32768 rows x 80 bf16 (335 MB, 5.9 TB/s; 62 us with one copy in flight).
+// 60 us for 32 planes x 32768 rows x 80 bf16 (335 MB, 5.6 TB/s; neighbours 61 us; 5 us more with one copy in flight).
 #include "elem16.cuh"
 #include "overlap.h"
 

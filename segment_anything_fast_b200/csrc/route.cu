@@ -7,9 +7,9 @@
 // tokens among those of their expert (a warp owns a run of pairs, ranks equal experts among its lanes with match_any and
 // keeps a running count per expert in shared memory); then (second launch, or after a barrier when one block is enough)
 // it adds up the counts of the blocks before it and places its pairs.  Nothing depends on the order in which atomics
-// arrive.  Bound by latency: 13.8 us for 32768 tokens x 64 experts, k = 4 (18.6 us with k rounds of maxima over eight lanes a
-// token, 34 us with a warp a token; two lanes a token 14.5 us; a second launch that starts early 0.3 to 0.5 us less,
-// which is not worth its own kind of dependency), 3.0 us for one token of 16 experts.
+// arrive.  Bound by latency: 14.5 us for 32768 tokens x 64 experts, k = 4, in a captured run (with k rounds of maxima over eight
+// lanes a token 5 us more, with a warp a token 20; with two lanes a token 0.7; a second launch that starts early 0.3 to 0.5 us
+// less, which is not worth its own kind of dependency), 3.8 us for one token of 16 experts.
 #include "common.cuh"
 
 namespace samb {

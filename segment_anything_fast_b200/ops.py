@@ -778,7 +778,7 @@ def route_topk(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] = None
                renorm: bool = True, scale: float = 1.0) -> Routing:
     """Router of a mixture of experts over fp32 ``logits [T, E]`` (E up to 512, k up to 8): every token's k largest
     logits (plus ``bias [E]``, which decides the choice only; ties to the lower index), their softmax or sigmoid
-    weights, and the order of the choices by expert for ``gemm_grouped`` and ``combine_topk``.  An expert at -inf or NaN
+    weights (the bias is added to the logit: one trained on top of the sigmoid or softmax orders experts differently), and the order of the choices by expert for ``gemm_grouped`` and ``combine_topk``.  An expert at -inf or NaN
     is never chosen: a token with nobody left (a padded one) gets id -1, weight 0 and no place."""
     dev = logits.get_device()
     if logits.dtype is not _F32 or dev < 0 or dev != torch.cuda.current_device():
@@ -857,7 +857,7 @@ def gemm_grouped(a: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows: 
     """Products grouped by expert: ``out[s] = act(a[rows[s]] @ w[e]^T + bias[e])`` for ``offsets[e] <= s < offsets[e + 1]``
     (without ``rows``: ``a[s]``), with ``a [M, K]`` and ``w [E, N, K]`` bfloat16 or float16, int32 ``offsets [E + 1]`` and
     ``rows [S]`` as ``route_topk`` gives them.  Rows of ``out [S, N]`` behind the last expert's are left as they were
-    (unspecified in a new ``out``); an index outside ``a`` stands for a row of zeros."""
+    (unspecified in a new ``out``); an index outside ``a`` (of one row at least) stands for a row of zeros."""
     dtype, dev = _half(a, "a")
     return _grouped("gemm_grouped", a, None, w, None, offsets, rows, bias, gelu, out, dtype, dev)
 
